@@ -58,6 +58,8 @@ for _g, _names in {
     "decay": "mlstm_scan ssd_scan",
     "streams": "stream_mix_norm stream_embed",
     "lnorm": "layer_norm_cast embed_layer_norm sandwich_norm_residual",
+    "keys": ("context_attention_weights paged_attention_weights heavy_keys "
+             "compact_pages"),
 }.items():
     for _n in _names.split():
         _OP_GROUP[_n] = _g
@@ -914,6 +916,165 @@ def context_attention(q: torch.Tensor, k_cache: torch.Tensor,
     return torch_ref.context_attention(q, k_cache, v_cache, cu_seqlens_q,
                                        kv_lens, block_tables, scale, window,
                                        sinks)
+
+
+# ---- a cache kept to a budget (kernel group "keys") -------------------------
+
+def _own_pages(k_cache, v_cache, key_weights, block_tables) -> None:
+    """What the operators on weighted pages ask of them, on any device."""
+    if k_cache.dim() != 4 or k_cache.size(2) != 16 \
+            or v_cache.shape != k_cache.shape \
+            or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache are [pages, kv heads, 16, "
+                         "head_dim] of one shape and type")
+    _weighted_pages(key_weights, block_tables)
+    if key_weights.shape != k_cache.shape[:3]:
+        raise ValueError(f"key_weights {tuple(key_weights.shape)} do not "
+                         f"belong to pages {tuple(k_cache.shape)}")
+    for t in (k_cache, v_cache):
+        if not t.is_contiguous():
+            raise ValueError("the caches have to be contiguous")
+
+
+def _weighted_pages(key_weights, block_tables) -> None:
+    if key_weights.dim() != 3 or key_weights.size(2) != 16 \
+            or key_weights.dtype != torch.float32 \
+            or not key_weights.is_contiguous():
+        raise ValueError("key_weights is contiguous f32 [pages, kv heads, 16]")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+        raise ValueError("block_tables is int32 [sequences, pages]")
+
+
+def _lengths_of(lens, block_tables, what: str) -> torch.Tensor:
+    if lens.dtype != torch.int32 or lens.dim() != 1 \
+            or lens.size(0) != block_tables.size(0):
+        raise ValueError(f"{what} is int32, one for each row of block_tables")
+    return lens.contiguous()
+
+
+def _query_rows(q, k_cache) -> torch.Tensor:
+    """q as the kernels read it: heads one behind another, rows in 16 bytes."""
+    if q.dim() != 3 or q.size(2) != k_cache.size(3) \
+            or q.size(1) % k_cache.size(1):
+        raise ValueError(f"q {tuple(q.shape)} does not belong to pages "
+                         f"{tuple(k_cache.shape)}")
+    D = q.size(2)
+    whole = q.stride(2) == 1 and q.stride(1) == D \
+        and (q.size(0) < 2 or q.stride(0) % 8 == 0) \
+        and q.data_ptr() % 16 == 0
+    return q if whole else q.contiguous()
+
+
+def context_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
+                              v_cache: torch.Tensor,
+                              key_weights: torch.Tensor,
+                              cu_seqlens_q: torch.Tensor,
+                              kv_lens: torch.Tensor,
+                              block_tables: torch.Tensor, scale: float,
+                              sinks: torch.Tensor | None = None,
+                              tiles=None) -> torch.Tensor:
+    """context_attention that also keeps how much weight every key receives.
+    key_weights [pages, kv heads, 16] f32 lies beside the cache's pages, in
+    place: a key's entry grows by its softmax weights, summed over the chunk's
+    rows that see it and the query heads of its kv head. The keys of the
+    chunk's own rows (the last of kv_lens) begin anew, so that a page's entries
+    need no clearing when it changes hands. A sequence without rows changes
+    nothing. Pages are a sequence's own here: what becomes of the weights of one
+    that two tables of a call share is not defined. q bf16 of any strides, head
+    sizes 64, 128 and 256, bf16 or e4m3 pages of 16 keys."""
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    kv_lens = _lengths_of(kv_lens, block_tables, "kv_lens")
+    if cu_seqlens_q.dtype != torch.int32 \
+            or cu_seqlens_q.shape != (block_tables.size(0) + 1,):
+        raise ValueError("cu_seqlens_q is int32, one more than block_tables' "
+                         "rows")
+    q = _query_rows(q, k_cache)
+    if q.is_cuda:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        cu = cu_seqlens_q.contiguous()
+        tile_seq, tile_qbase = tiles or _build_tiles(cu)
+        _K.context_attention_weights(
+            out, q, k_cache, v_cache, key_weights, tile_seq, tile_qbase, cu,
+            kv_lens, block_tables.contiguous(), scale,
+            _sinks_arg(sinks, q.device))
+        return out
+    return torch_ref.context_attention_weights(
+        q, k_cache, v_cache, key_weights, cu_seqlens_q, kv_lens, block_tables,
+        scale, sinks)
+
+
+def paged_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, key_weights: torch.Tensor,
+                            block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, scale: float,
+                            sinks: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention that also keeps how much weight every key receives, as
+    context_attention_weights does: one row per sequence, whose own key is the
+    last of seq_lens and begins anew. Rows of no keys come out as zeros. The
+    scores are kept in f32 in between: 64 bytes for each row, query head and
+    page of the table's width."""
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    seq_lens = _lengths_of(seq_lens, block_tables, "seq_lens")
+    if q.size(0) != block_tables.size(0):
+        raise ValueError("q has one row for each row of block_tables")
+    q = _query_rows(q, k_cache)
+    if q.is_cuda:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _K.paged_attention_weights(
+            out, q, k_cache, v_cache, key_weights, block_tables.contiguous(),
+            seq_lens, scale, _sinks_arg(sinks, q.device))
+        return out
+    return torch_ref.paged_attention_weights(
+        q, k_cache, v_cache, key_weights, block_tables, seq_lens, scale, sinks)
+
+
+def heavy_keys(key_weights: torch.Tensor, block_tables: torch.Tensor,
+               seq_lens: torch.Tensor, budget: int, recent: int):
+    """The keys that stay when every sequence's cache is cut to `budget` keys:
+    its newest `recent` and, of the others, those whose weights, summed over
+    the kv heads (in f64, then rounded to f32), are largest; equal ones go by
+    the lower place, a NaN is larger than every number. Returns (kept
+    [sequences, budget] int32, their places in ascending order, -1 behind the
+    last; how many they are [sequences] int32). A sequence of up to `budget`
+    keys keeps them all."""
+    _weighted_pages(key_weights, block_tables)
+    seq_lens = _lengths_of(seq_lens, block_tables, "seq_lens")
+    if not 0 <= recent <= budget or budget < 1:
+        raise ValueError(f"a budget of {budget} keys cannot hold the newest "
+                         f"{recent}")
+    if key_weights.is_cuda:
+        B = block_tables.size(0)
+        kept = torch.empty(B, budget, dtype=torch.int32,
+                           device=key_weights.device)
+        kept_lens = torch.empty(B, dtype=torch.int32,
+                                device=key_weights.device)
+        _K.heavy_keys(kept, kept_lens, key_weights, block_tables.contiguous(),
+                      seq_lens, budget, recent)
+        return kept, kept_lens
+    return torch_ref.heavy_keys(key_weights, block_tables, seq_lens, budget,
+                                recent)
+
+
+def compact_pages(k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  key_weights: torch.Tensor, block_tables: torch.Tensor,
+                  kept: torch.Tensor, kept_lens: torch.Tensor) -> None:
+    """Closes the gaps that heavy_keys left, in place: key kept[b, i] of
+    sequence b goes to place i, K, V and weights, for i below kept_lens[b].
+    `kept` ascends; places at and behind kept_lens[b] stay as they were, and
+    the pages behind it can be given back. Pages are a sequence's own: no page
+    may be in two tables."""
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    kept_lens = _lengths_of(kept_lens, block_tables, "kept_lens")
+    if kept.dtype != torch.int32 or kept.dim() != 2 \
+            or kept.size(0) != block_tables.size(0):
+        raise ValueError("kept is int32 [sequences, places]")
+    if k_cache.is_cuda:
+        _K.compact_pages(k_cache, v_cache, key_weights,
+                         block_tables.contiguous(), kept.contiguous(),
+                         kept_lens)
+        return
+    torch_ref.compact_pages(k_cache, v_cache, key_weights, block_tables, kept,
+                            kept_lens)
 
 
 def gelu_and_mul(x: torch.Tensor) -> torch.Tensor:

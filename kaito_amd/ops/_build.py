@@ -57,6 +57,9 @@ GROUPS: Dict[str, List[str]] = {
     "streams": ["streams.hip"],
     # layer norms around sub-layers on an f32 residual stream
     "lnorm": ["layer_norm_f32.hip"],
+    # a cache kept to a budget: attention that keeps the keys' weights, the
+    # choice of the keys that stay, the closing of the gaps
+    "keys": ["context_weights.hip", "paged_weights.hip", "key_eviction.hip"],
 }
 
 

@@ -85,6 +85,7 @@ struct Args {
   int db_n;
   float temp_coef;
   int temp_every;
+  float2* stats;                    // STATS: [T, QH] maximum (log2 domain), 1 / sum
 };
 
 // LDS serves 256 bytes per cycle, 16 lanes of a 16-byte read, 32 of an 8-byte
@@ -140,9 +141,10 @@ constexpr int kvt() { return D + DV <= 320 ? 64 : 32; }
 // D1: dims of q and k that come from q/k; the others come from q2/k2. KVT: keys
 // per tile; NW: waves of 32 rows.
 // EXT: capping, penalty, kept first keys, chunked mask, head gate, and
-// softmax weights that enter P.V as a bf16 value + remainder pair.
+// softmax weights that enter P.V as a bf16 value + remainder pair. STATS: every
+// row's maximum and sum are kept, for a second pass over its weights.
 template <int D, int DV, int SRC, bool EXT, bool SIG = false, bool DB = false,
-          int D1 = D, int KVT = kvt<D, DV>(), int NW = 4>
+          int D1 = D, int KVT = kvt<D, DV>(), int NW = 4, bool STATS = false>
 __global__ __launch_bounds__(NW * 64, (D + DV > 384 ? 1 : 2))
 void flash_prefill_kernel(const Args a) {
   constexpr int NK = KVT / 32, KK = D / 16, NS = KVT / 16, DT = DV / 32;
@@ -584,6 +586,8 @@ void flash_prefill_kernel(const Args a) {
   l = SIG ? 1.0f : l + __shfl_xor(l, 32, 64);
   if (qrow >= q_len) return;
   float inv = 1.0f / fmaxf(l, 1e-30f);
+  if constexpr (STATS)
+    if (h == 0) a.stats[(int64_t)(tok0 + qrow) * a.QH + head] = {m, inv};
   if (EXT && a.gate) {
     const float g =
         bf16_to_f32(a.gate[(int64_t)(tok0 + qrow) * a.gate_s0 + head]);

@@ -95,8 +95,15 @@ struct DecodeArgs {
   int64_t k_stride, v_stride;
   const float* cos_sin;             // [positions, D]
   const int64_t* slots;             // [T]
+  // KEEP: scores (log2 domain), and what makes weights of them
+  float* scores;                    // [T, QH, score_stride]
+  int64_t score_stride;             // a multiple of KT that holds the table's keys
+  float2* stats;                    // [T, QH] maximum, 1 / sum
 
-  template <bool BIASED> KAITO_DEV int len(const int64_t row) const {
+  // KEEP writes per key: never more of them than the table holds
+  template <bool BIASED, bool KEEP = false>
+  KAITO_DEV int len(const int64_t row) const {
+    if constexpr (KEEP) return min(seq_lens[row], max_blocks * BS);
     return BIASED ? (int)positions[row] + 1 : seq_lens[row];
   }
 };
@@ -217,7 +224,8 @@ KAITO_DEV Spans spans_of(const int seq_len, const int window, const int nsplit,
   return p;
 }
 
-template <int D, bool FP8, int NW, bool SPLIT, bool BIASED, bool ROPE>
+template <int D, bool FP8, int NW, bool SPLIT, bool BIASED, bool ROPE,
+          bool KEEP = false>
 __global__ __launch_bounds__(NW * 64, NW <= 4 && D <= 128 ? 3 : 2)
 void paged_decode_kernel(const DecodeArgs a) {
   constexpr int KK = D / 32;        // 16x16x32 steps over the dims
@@ -248,7 +256,7 @@ void paged_decode_kernel(const DecodeArgs a) {
         a.out[((int64_t)seq * QH + kvh * a.G) * D + i] = 0;
     return;
   }
-  const int seq_len = a.len<BIASED>(seq);
+  const int seq_len = a.len<BIASED, KEEP>(seq);
   const int* bt = a.block_tables + (int64_t)table * a.max_blocks;
 
   const int nsplit = SPLIT ? gridDim.y : 1, split = SPLIT ? blockIdx.y : 0;
@@ -427,6 +435,16 @@ void paged_decode_kernel(const DecodeArgs a) {
           if (!seen(i, r)) s[i][r] = NONE;
           mx = fmaxf(mx, s[i][r]);
         }
+      if constexpr (KEEP) {
+        if (lo < a.G) {
+          float* at = a.scores +
+              ((int64_t)seq * QH + kvh * a.G + lo) * a.score_stride + key0 +
+              4 * hi;
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            *reinterpret_cast<f32x4*>(at + 16 * i) = s[i];
+        }
+      }
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       if (__any(mx > m)) {
@@ -562,6 +580,9 @@ void paged_decode_kernel(const DecodeArgs a) {
       if (d == 0) { row[D] = gm; row[D + 1] = den; }
     } else {
       if (a.sinks) den += fold_weight<BIASED>(sink, gm);
+      if constexpr (KEEP)
+        if (d == 0)
+          a.stats[(int64_t)seq * QH + head] = {gm, 1.f / fmaxf(den, 1e-20f)};
       store_head<BIASED>(a, seq, QH, head, D, d, num, den);
     }
   }
@@ -570,13 +591,13 @@ void paged_decode_kernel(const DecodeArgs a) {
 // One workgroup per (sequence, head) folds the splits that had keys, unless
 // the first had them all. A chain of loads, so a short one: lane s of every
 // wave has split s's weight.
-template <int D, bool BIASED>
+template <int D, bool BIASED, bool KEEP = false>
 __global__ __launch_bounds__(D)
 void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
   const int64_t row = blockIdx.x, rows = gridDim.x;
   if (BIASED && a.token_seq[row / QH] < 0) return;
   const int used =
-      spans_of(a.len<BIASED>(row / QH), a.window, splits, WIDE).used;
+      spans_of(a.len<BIASED, KEEP>(row / QH), a.window, splits, WIDE).used;
   if (used == 1) return;
   constexpr float NONE = BIASED ? -INFINITY : -1e30f;
   const int d = threadIdx.x, lane = d & 63;
@@ -592,6 +613,8 @@ void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
   const float e = lane < used ? fold_weight<BIASED>(m, gm) : 0.f;
   float den = wave_reduce_sum(e * l);
   if (a.sinks) den += fold_weight<BIASED>(sink, gm);
+  if constexpr (KEEP)
+    if (d == 0) a.stats[row] = {gm, 1.f / fmaxf(den, 1e-20f)};
   float num = 0.f;
 #pragma unroll 4
   for (int s = 0; s < used; s++)
@@ -601,7 +624,7 @@ void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
   store_head<BIASED>(a, row / QH, QH, (int)(row % QH), D, d, num, den);
 }
 
-template <int D, bool FP8, bool BIASED, bool ROPE = false>
+template <int D, bool FP8, bool BIASED, bool ROPE = false, bool KEEP = false>
 void launch_paged_decode(DecodeArgs a, const at::Tensor& out, int T) {
   auto stream = at::hip::getCurrentHIPStream();
   const int64_t pairs = (int64_t)T * a.KH;
@@ -629,7 +652,7 @@ void launch_paged_decode(DecodeArgs a, const at::Tensor& out, int T) {
   int64_t longest = (int64_t)a.max_blocks * BS;
   if (a.window > 0) longest = std::min<int64_t>(longest, a.window + BS);
 #define PA_LAUNCH(NW_, SPLIT_, GRID_)                                         \
-  hipLaunchKernelGGL((paged_decode_kernel<D, FP8, NW_, SPLIT_, BIASED, ROPE>), GRID_, \
+  hipLaunchKernelGGL((paged_decode_kernel<D, FP8, NW_, SPLIT_, BIASED, ROPE, KEEP>), GRID_, \
                      dim3(NW_ * 64), 0, stream, a)
   const int64_t splits = std::min<int64_t>(
       {SPLIT_FILL / pairs, longest / (WIDE * KT * SPLIT_MIN), 64});
@@ -639,7 +662,7 @@ void launch_paged_decode(DecodeArgs a, const at::Tensor& out, int T) {
                                 out.options().dtype(at::kFloat));
     a.part = part.data_ptr<float>();
     PA_LAUNCH(WIDE, true, dim3(pairs, splits));
-    hipLaunchKernelGGL((paged_fold_kernel<D, BIASED>), dim3(T * a.KH * a.G),
+    hipLaunchKernelGGL((paged_fold_kernel<D, BIASED, KEEP>), dim3(T * a.KH * a.G),
                        dim3(D), 0, stream, a, a.KH * a.G, (int)splits);
   } else if (pairs <= (D <= 64 ? 512 : 256)) {
     PA_LAUNCH(WIDE, false, dim3(pairs));

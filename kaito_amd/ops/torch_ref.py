@@ -204,6 +204,103 @@ def context_attention(q: torch.Tensor, k_cache: torch.Tensor,
     return out
 
 
+def _add_key_weights(key_weights, block_table, L: int, new: int, p):
+    """p [QH, rows, L]: adds its sums over rows and the heads of a group to
+    the first L keys' entries; the last `new` of them begin anew."""
+    KH, BS = key_weights.shape[1:]
+    j = torch.arange(L, device=p.device)
+    pages = block_table[j // BS].long()
+    old = key_weights[pages, :, j % BS]                            # [L, KH]
+    old[L - new:] = 0
+    w = p.unflatten(0, (KH, -1)).sum((1, 2)).T
+    key_weights[pages, :, j % BS] = old + w.to(key_weights.dtype)
+
+
+def context_attention_weights(q, k_cache, v_cache, key_weights, cu_seqlens_q,
+                              kv_lens, block_tables, scale: float, sinks=None):
+    """context_attention whose weights are added to key_weights [NB, KH, BS],
+    in place; the keys of a chunk's own rows begin anew."""
+    T, QH, D = q.shape
+    KH, BS = k_cache.shape[1:3]
+    k_cache, v_cache = (
+        t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t
+        for t in (k_cache, v_cache))
+    out = torch.zeros_like(q)
+    cs = cu_seqlens_q.tolist()
+    for b in range(len(cs) - 1):
+        n = cs[b + 1] - cs[b]
+        L = min(int(kv_lens[b]), block_tables.size(1) * BS)
+        if n == 0:
+            continue
+        j = torch.arange(L, device=q.device)
+        pages = block_tables[b, j // BS].long()
+        k = k_cache[pages, :, j % BS].float()                  # [L, KH, D]
+        v = v_cache[pages, :, j % BS].float()
+        k, v = (t.repeat_interleave(QH // KH, 1).transpose(0, 1)
+                for t in (k, v))
+        s = (q[cs[b]:cs[b + 1]].float().transpose(0, 1)
+             @ k.transpose(1, 2)) * scale                      # [QH, n, L]
+        later = j > torch.arange(L - n, L, device=q.device)[:, None]
+        s = s.masked_fill(later, float("-inf"))
+        if sinks is not None:
+            s = torch.cat([s, sinks.float()[:, None, None].expand(-1, n, 1)],
+                          dim=-1)
+        p = torch.softmax(s, dim=-1)[..., :L]
+        out[cs[b]:cs[b + 1]] = (p @ v).transpose(0, 1).to(q.dtype)
+        _add_key_weights(key_weights, block_tables[b], L, n, p)
+    return out
+
+
+def paged_attention_weights(q, k_cache, v_cache, key_weights, block_tables,
+                            seq_lens, scale: float, sinks=None):
+    """context_attention_weights of one row per sequence; a row of no keys
+    comes out as zeros."""
+    live = (seq_lens > 0).nonzero().flatten()
+    out = torch.zeros_like(q)
+    cu = torch.arange(len(live) + 1, dtype=torch.int32)
+    out[live] = context_attention_weights(
+        q[live], k_cache, v_cache, key_weights, cu, seq_lens[live],
+        block_tables[live], scale, sinks)
+    return out
+
+
+def heavy_keys(key_weights, block_tables, seq_lens, budget: int, recent: int):
+    """(kept [B, budget], kept_lens [B]): the newest `recent` keys of each
+    sequence and the others of the largest sums over the kv heads."""
+    BS = key_weights.size(2)
+    kept = torch.full((block_tables.size(0), budget), -1, dtype=torch.int32,
+                      device=key_weights.device)
+    n = seq_lens.clamp(0, block_tables.size(1) * BS)
+    for b, L in enumerate(n.tolist()):
+        j = torch.arange(L, device=key_weights.device)
+        if L > budget:
+            old, pages = j[:L - recent], block_tables[b, j // BS].long()
+            w = key_weights[pages, :, j % BS].double().sum(1).float()
+            order = w[old].sort(descending=True, stable=True).indices
+            j = torch.cat([order[:budget - recent].sort().values,
+                           j[L - recent:]])
+        kept[b, :len(j)] = j.int()
+    return kept, n.clamp(max=budget).int()
+
+
+def compact_pages(k_cache, v_cache, key_weights, block_tables, kept,
+                  kept_lens):
+    """Key kept[b, i] goes to place i of its sequence, in place; places and
+    pages that are none are left out."""
+    NB, _, BS = key_weights.shape
+    most = min(kept.size(1), block_tables.size(1) * BS)
+    for b, n in enumerate(kept_lens.clamp(0, most).tolist()):
+        i = torch.arange(n, device=kept.device)
+        src, t = kept[b, :n].long(), block_tables[b].long()
+        real = (src >= 0) & (src < len(t) * BS)
+        i, src = i[real], src[real]
+        pages = torch.stack([t[src // BS], t[i // BS]])
+        real = ((pages >= 0) & (pages < NB)).all(0)
+        i, src = i[real], src[real]
+        for x in (k_cache, v_cache, key_weights):
+            x[t[i // BS], :, i % BS] = x[t[src // BS], :, src % BS]
+
+
 def w4a16_unpack(qweight: torch.Tensor, scales: torch.Tensor,
                  zeros: torch.Tensor, group: int) -> torch.Tensor:
     """Dequantize the native W4A16 layout (qweight u32 [N, K/8], 8

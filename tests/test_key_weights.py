@@ -1,0 +1,352 @@
+"""A cache kept to a budget: attention that keeps what every key receives, the
+choice of the keys that stay and the closing of the gaps, against plain loops in 64
+bits.
+
+Tolerances. Outputs are bf16: half a step is 2^-8 of the value. Chunks' weights go
+into the product with V as bf16, which adds 2^-8 of sum p |v|; single tokens' go in
+whole. A score is a sum of D products in f32, off by at most (D + 2) 2^-24 of the
+sum of their sizes, twice that for a weight (its own and its row's sum), and e4m3
+and bf16 operands are exact. A key's entry is a sum of such weights and its old
+value, each step of which rounds to 2^-24; 2^-20 of it covers the exponential, the
+reciprocal and up to a few thousand additions of a random sign."""
+import math
+
+import pytest
+import torch
+
+from kaito_amd import ops
+
+CPU_OR_GPU = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+PAGE = 16
+
+
+def _pages(lens, KH, D, fp8=False, width=None, seed=0):
+    """Caches and tables of sequences of `lens` keys, in pages of no order; what
+    no sequence owns holds NaN (in e4m3 0x7f is one)."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // PAGE) for n in lens]
+    width = max(width or 0, max(need + [1]))
+    perm = torch.randperm(sum(need) + 2, generator=g).int()
+    tables = torch.full((len(lens), width), int(perm[-1]), dtype=torch.int32)
+    shape = (len(perm), KH, PAGE, D)
+    k, v = (torch.full(shape, math.nan) for _ in range(2))
+    w = torch.full(shape[:3], math.nan)
+    at = 0
+    for b, n in enumerate(lens):
+        tables[b, :need[b]] = perm[at:at + need[b]]
+        at += need[b]
+        for i in range(0, n, PAGE):
+            p, m = tables[b, i // PAGE], min(PAGE, n - i)
+            k[p, :, :m] = torch.randn(KH, m, D, generator=g)
+            v[p, :, :m] = torch.randn(KH, m, D, generator=g)
+            w[p, :, :m] = torch.rand(KH, m, generator=g) ** 3 * 5
+    if fp8:
+        k, v = (t.to(torch.float8_e4m3fn).view(torch.uint8) for t in (k, v))
+    else:
+        k, v = k.bfloat16(), v.bfloat16()
+    return k, v, w, tables
+
+
+def _f64(cache):
+    x = cache.cpu()
+    return (x.view(torch.float8_e4m3fn) if x.dtype == torch.uint8 else x).double()
+
+
+def _oracle(q, k, v, w, new, lens, tables, scale, sinks):
+    """(output, its tolerance without its own rounding, weights, their
+    tolerance) in 64 bits."""
+    k, v, q, w = _f64(k), _f64(v), q.cpu().double(), w.cpu().double()
+    KH, D = k.size(1), k.size(3)
+    G = q.size(1) // KH
+    out, near = torch.zeros_like(q), torch.zeros_like(q)
+    off = torch.zeros_like(w)
+    at = 0
+    for b, (n, L) in enumerate(zip(new, lens)):
+        if n == 0 or L == 0:
+            at += n
+            continue
+        j = torch.arange(L)
+        p = tables[b].cpu().long()[j // PAGE]
+        kb, vb = k[p, :, j % PAGE], v[p, :, j % PAGE]              # [L, KH, D]
+        later = j > torch.arange(L - n, L)[:, None]
+        gain, gain_off = torch.zeros(L, KH).double(), torch.zeros(L, KH).double()
+        for h in range(G * KH):
+            x = q[at:at + n, h]
+            s = (x @ kb[:, h // G].T * scale).masked_fill(later, -math.inf)
+            top = s.amax(1, keepdim=True)
+            if sinks is not None:
+                top = top.maximum(sinks[h].double())
+            e = (s - top).exp()
+            den = e.sum(1, keepdim=True)
+            if sinks is not None:
+                den = den + (sinks[h].double() - top).exp()
+            e = e / den
+            out[at:at + n, h] = e @ vb[:, h // G]
+            near[at:at + n, h] = e @ vb[:, h // G].abs()
+            gain[:, h // G] += e.sum(0)
+            size = (x.abs() @ kb[:, h // G].abs().T).amax(1) * abs(scale)
+            rel = 2 * (D + 2) * 2.0 ** -24 * size + 2.0 ** -20
+            gain_off[:, h // G] += (e * rel[:, None]).sum(0)
+        old = w[p, :, j % PAGE]
+        old[L - n:] = 0
+        w[p, :, j % PAGE] = old + gain
+        off[p, :, j % PAGE] = gain_off + (old + gain) * 2.0 ** -20
+        at += n
+    return out, near, w, off
+
+
+def _run(dev, layout, new, past, fp8=False, sinks=False, width=None, token=False,
+         seed=0):
+    QH, KH, D = layout
+    lens = [a + b for a, b in zip(new, past)]
+    k, v, w, tables = _pages(lens, KH, D, fp8, width, seed)
+    for b, (n, L) in enumerate(zip(new, lens)):    # what the slot's last user left
+        for j in range(L - n, L):
+            w[tables[b, j // PAGE], :, j % PAGE] = (math.nan, 3e38)[j % 2]
+    g = torch.Generator().manual_seed(seed + 1)
+    # rows cut from a fused projection
+    q = torch.randn(sum(new), QH * D + 64, generator=g).mul(2).bfloat16().to(dev)
+    q = q[:, :QH * D].unflatten(1, (QH, D))
+    s = torch.randn(QH, generator=g) if sinks else None
+    scale = D ** -0.5
+    want, near, want_w, off = _oracle(q, k, v, w, new, lens, tables, scale, s)
+    k, v, got_w, tables, lens_t = (
+        t.to(dev) for t in (k, v, w, tables, torch.tensor(lens, dtype=torch.int32)))
+    s = s.to(dev) if sinks else None
+    if token:
+        out = ops.paged_attention_weights(q, k, v, got_w, tables, lens_t, scale, s)
+    else:
+        cu = torch.tensor([0] + new).cumsum(0).int().to(dev)
+        out = ops.context_attention_weights(q, k, v, got_w, cu, lens_t, tables,
+                                            scale, s)
+    out, got_w = out.cpu().double(), got_w.cpu().double()
+    bf16 = 2.0 ** -8
+    room = bf16 * want.abs() + (near * (2.0 ** -14 if token else bf16)) + 2.0 ** -20
+    assert ((out - want).abs() <= room).all(), ((out - want).abs() - room).max()
+    live = off > 0
+    assert ((got_w - want_w).abs() <= off)[live].all()
+    # nothing else has changed
+    assert torch.equal(got_w[~live].float().view(torch.int32),
+                       w[~live].view(torch.int32))
+
+
+LAYOUTS = [(4, 1, 64), (8, 1, 64), (2, 2, 64), (8, 2, 128), (7, 1, 128),
+           (3, 3, 128), (4, 2, 256), (4, 1, 256)]
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_chunks(dev, layout, fp8):
+    """Edges of the 32- and 64-row tiles, of pages and of 64 and 256 keys;
+    prompts whole and behind a past, and a sequence without rows."""
+    _run(dev, layout, [1, 0, 17, 64, 33, 65, 5], [0, 40, 0, 1, 223, 191, 252],
+         fp8=fp8, sinks=not fp8, width=24)
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("layout", [(8, 2, 128), (5, 1, 128), (2, 1, 256)])
+def test_long_chunks(dev, layout):
+    _run(dev, layout, [300, 129], [700, 0], sinks=True, seed=3)
+
+
+@pytest.mark.gpu
+def test_chunk_over_many_keys():
+    _run("cuda", (4, 1, 128), [70], [9000])
+    _run("cuda", (16, 2, 64), [1030], [3], fp8=True)
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tokens(dev, layout, fp8):
+    lens = [1, 15, 16, 17, 31, 32, 33, 0, 64, 65, 127, 129, 300]
+    new = [1] * len(lens)
+    _run(dev, layout, new, [n - 1 for n in lens], fp8=fp8, sinks=not fp8,
+         token=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,KH,lens,width", [
+    (128, 8, [40, 200, 7] * 11, 13),          # pairs beyond a workgroup per CU
+    (128, 2, [1900, 33, 0, 2047], 128),       # few pairs, a long table: splits
+    (128, 1, [5000], 700), (256, 1, [700, 3], 200),
+    (64, 8, [17], 4096),                      # splits that are all but one empty
+    (64, 8, [30, 5, 64, 70] * 40, 5),
+    (128, 8, [64] * 140, 4),                  # two waves per pair
+])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_token_launch_rules(D, KH, lens, width, fp8):
+    _run("cuda", (4 * KH, KH, D), [1] * len(lens), [n - 1 for n in lens], fp8=fp8,
+         sinks=fp8, width=width, token=True)
+
+
+@pytest.mark.gpu
+def test_scores_without_a_weight():
+    """Keys whose scores are minus infinity receive nothing, and a row that has
+    no other key changes no entry."""
+    k, v, w, t = _pages([20, 4], 1, 64)
+    v[v.isnan()] = 0
+    q = torch.ones(2, 1, 64).bfloat16()
+    k[t[0, 0], :, 3] = -3e38                  # -3e38 * 64 ones
+    k[t[1, 0], :, :4] = -3e38
+    lens = torch.tensor([20, 4], dtype=torch.int32)
+    args = [x.to("cuda") for x in (q, k, v)]
+    for op in (ops.paged_attention_weights, ops.context_attention_weights):
+        got = w.to("cuda")
+        more = (torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"),) \
+            if op is ops.context_attention_weights else ()
+        rows = (t.to("cuda"), lens.to("cuda"))
+        op(*args, got, *more, *(rows[::-1] if more else rows), 1.0)
+        got = got.cpu()
+        assert got[t[0, 0], 0, 3] == w[t[0, 0], 0, 3]
+        assert torch.equal(got[t[1, 0], 0, :3], w[t[1, 0], 0, :3])
+        assert got[t[1, 0], 0, 3] == 0        # its own key: anew, and nothing
+
+
+def _heavy(w, tables, lens, budget, recent):
+    """The rule, key by key."""
+    kept = torch.full((len(lens), budget), -1, dtype=torch.int32)
+    for b, L in enumerate(lens):
+        places = list(range(L))
+        if L > budget:
+            total = [float(w[tables[b, j // PAGE], :, j % PAGE].double().sum()
+                           .float()) for j in range(L - recent)]
+            order = sorted(range(L - recent), key=lambda j: (
+                -math.inf if math.isnan(total[j]) else -total[j], j))
+            places = sorted(order[:budget - recent]) + places[L - recent:]
+        kept[b, :len(places)] = torch.tensor(places, dtype=torch.int32)
+    return kept
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("budget,recent", [(1, 0), (1, 1), (64, 0), (64, 64),
+                                           (100, 37), (257, 16), (600, 5)])
+@pytest.mark.parametrize("kind", ["spread", "equal", "few", "zero", "signs"])
+def test_heavy_keys(dev, budget, recent, kind):
+    lens = [0, 1, 63, 64, 65, 100, 101, 258, 513]
+    _, _, w, tables = _pages(lens, 3, 64, width=40)
+    w = torch.nan_to_num(w, 7.)
+    if kind == "equal":
+        w.fill_(0.3)
+    if kind == "few":                      # many ties of three values
+        w = (w * 0.5).floor()
+    if kind == "zero":
+        w = w * 0 * torch.where(torch.rand(w.shape) < 0.5, 1., -1.)
+    if kind == "signs":
+        w = torch.where(torch.rand(w.shape) < 0.5, w, -w)
+        w[tables[8, 0], 0, 3] = math.nan
+        w[tables[8, 1], 1, 4] = math.inf
+        w[tables[8, 1], 1, 5] = -math.inf
+    kept, n = ops.heavy_keys(w.to(dev), tables.to(dev),
+                             torch.tensor(lens, dtype=torch.int32, device=dev),
+                             budget, recent)
+    assert torch.equal(kept.cpu(), _heavy(w, tables, lens, budget, recent))
+    assert n.tolist() == [min(L, budget) for L in lens]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,budget,recent", [([40000, 39999], 20000, 100),
+                                                ([70001], 1000, 999),
+                                                ([70001], 65537, 0)])
+def test_heavy_keys_of_long_caches(lens, budget, recent):
+    _, _, w, tables = _pages([1], 2, 64)
+    pages = -(-max(lens) // PAGE)
+    w = torch.rand(pages * len(lens), 2, PAGE)
+    w[::3] = 0.5                           # ties among them
+    tables = torch.randperm(len(w)).int().view(len(lens), pages)
+    kept, n = ops.heavy_keys(w.cuda(), tables.cuda(),
+                             torch.tensor(lens, dtype=torch.int32).cuda(), budget,
+                             recent)
+    assert torch.equal(kept.cpu(), _heavy(w, tables, lens, budget, recent))
+    assert n.tolist() == [budget] * len(lens)
+
+
+def _close(k, v, w, tables, kept, lens):
+    for b, n in enumerate(lens):
+        for x in (k, v, w):
+            rows = [x[tables[b, j // PAGE], :, j % PAGE].clone()
+                    for j in kept[b, :n].tolist()]
+            for i, row in enumerate(rows):
+                x[tables[b, i // PAGE], :, i % PAGE] = row
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("KH,D,fp8", [(1, 32, False), (2, 64, False), (3, 64, True),
+                                      (2, 128, False), (1, 256, True),
+                                      (2, 256, False)])
+def test_compact_pages(dev, KH, D, fp8):
+    """Bit for bit, the places behind the kept ones among them."""
+    lens = [500, 0, 1, 17, 300, 64]
+    k, v, w, tables = _pages(lens, KH, D, fp8, width=33)
+    kept = torch.full((6, 260), -1, dtype=torch.int32)
+    g = torch.Generator().manual_seed(5)
+    stay = [260, 0, 1, 9, 259, 64]
+    for b, (n, L) in enumerate(zip(stay, lens)):
+        kept[b, :n] = torch.randperm(L, generator=g)[:n].sort().values.int()
+    kept[4, :259] = torch.arange(41, 300).int()         # all move by 41
+    got = [t.to(dev) for t in (k, v, w)]
+    ops.compact_pages(*got, tables.to(dev), kept.to(dev),
+                      torch.tensor(stay, dtype=torch.int32, device=dev))
+    _close(k, v, w, tables, kept, stay)
+    for a, b in zip(got, (k, v, w)):
+        assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+def test_compact_pages_of_no_page(dev):
+    """Places and pages that are none are left out: nothing is read or written
+    for them."""
+    k, v, w, tables = _pages([100], 1, 64)
+    kept = torch.tensor([[-1, 2, 7, 5000, 60, 99]], dtype=torch.int32)
+    tables[0, 3] = 1 << 20                               # of key 60
+    tables[0, 6] = -5                                    # of key 99
+    got = [t.to(dev) for t in (k, v, w)]
+    ops.compact_pages(*got, tables.to(dev), kept.to(dev),
+                      torch.tensor([6], dtype=torch.int32, device=dev))
+    for x in (k, v, w):
+        rows = x[tables[0, 0], :, [2, 7]].clone()
+        x[tables[0, 0], :, [1, 2]] = rows
+    for a, b in zip(got, (k, v, w)):
+        assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+def test_refusals(dev):
+    k, v, w, t = (x.to(dev) for x in _pages([40], 2, 64))
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=dev)
+    n = torch.tensor([40], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    kept = torch.zeros(1, 8, dtype=torch.int32, device=dev)
+
+    def refused(f, *args):
+        with pytest.raises((ValueError, RuntimeError)):
+            f(*args)
+
+    token, chunk = ops.paged_attention_weights, ops.context_attention_weights
+    for bad in (w[:1], w.double(), w[:, :1], w.transpose(0, 1), w[:, :, :8]):
+        refused(token, q, k, v, bad, t, n, 1.0)
+        refused(chunk, q, k, v, bad, cu, n, t, 1.0)
+        refused(ops.compact_pages, k, v, bad, t, kept, n)
+    for bad in (q[:, :3], q[..., :32], q[0], torch.zeros(2, 4, 64).to(q)):
+        refused(token, bad, k, v, w, t, n, 1.0)
+    refused(chunk, q[:, :3], k, v, w, cu, n, t, 1.0)
+    refused(token, q, k, v[:, :, :, :32], w, t, n, 1.0)
+    refused(token, q, k, v.view(torch.uint8), w, t, n, 1.0)
+    refused(token, q, k, v, w, t.long(), n, 1.0)
+    refused(token, q, k, v, w, t, n.long(), 1.0)
+    refused(token, q, k, v, w, t, n[:0], 1.0)
+    refused(chunk, q, k, v, w, cu[:1], n, t, 1.0)
+    refused(chunk, q, k, v, w, cu.long(), n, t, 1.0)
+    for budget, recent in ((0, 0), (8, 9), (8, -1), (-4, -4)):
+        refused(ops.heavy_keys, w, t, n, budget, recent)
+    refused(ops.heavy_keys, w, t, n[:0], 8, 0)
+    refused(ops.compact_pages, k, v, w, t, kept.long(), n)
+    refused(ops.compact_pages, k, v, w, t, kept[:0], n)
+    refused(ops.compact_pages, k.transpose(2, 3), v, w, t, kept, n)
+    if dev == "cuda":
+        refused(token, q.float(), k, v, w, t, n, 1.0)
+        refused(token, q, k, v, w, t.cpu(), n, 1.0)
+        refused(token, q, k, v, w, t, n, 1.0, torch.zeros(3, device=dev))
+        refused(ops.heavy_keys, w, t, n.cpu(), 8, 0)
+        refused(ops.compact_pages, k, k, w, t, kept, n)
