@@ -46,16 +46,52 @@ void key_total_kernel(unsigned* __restrict__ totals,      // [B, width * 16]
 }
 
 constexpr int CHOOSERS = 1024;
+constexpr int BINS = 2 * CHOOSERS;
+constexpr int FEW = 64;             // totals whose order one wave finds
 
+// x combined over the lanes up to this one; 0 is what changes nothing
+template <typename F>
+KAITO_DEV unsigned lanes_up_to(unsigned x, F f) {
+#define SCAN_STEP(CTRL_, ROWS_)                                               \
+  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL_, ROWS_, 0xf, \
+                                                 false))
+  SCAN_STEP(0x111, 0xf);            // row_shr 1, 2, 4, 8
+  SCAN_STEP(0x112, 0xf);
+  SCAN_STEP(0x114, 0xf);
+  SCAN_STEP(0x118, 0xf);
+  SCAN_STEP(0x142, 0xa);            // the last lane of a row to the next row
+  SCAN_STEP(0x143, 0xc);            // and of the first half to the second
+#undef SCAN_STEP
+  return x;
+}
+struct Plus {
+  KAITO_DEV unsigned operator()(unsigned a, unsigned b) const { return a + b; }
+};
+struct Larger {
+  KAITO_DEV unsigned operator()(unsigned a, unsigned b) const { return max(a, b); }
+};
+
+// how many of a ballot's lanes come before this one
+KAITO_DEV int lanes_below(const unsigned long long b) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((unsigned)b, 0));
+}
+
+// PER: keys of a thread that stay in its registers; ONE: these are all; SUMS: their
+// totals are made here
+template <int PER, bool ONE, bool SUMS>
 __global__ __launch_bounds__(CHOOSERS)
 void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
                         const unsigned* __restrict__ totals,
+                        const float* __restrict__ key_weights,
+                        const int* __restrict__ block_tables,
                         const int* __restrict__ seq_lens, const int width,
-                        const int budget, const int recent) {
-  constexpr int WAVES = CHOOSERS / 64;
-  __shared__ int hist[256];
-  __shared__ int found[2];
-  __shared__ int counts[2][WAVES];
+                        const int KH, const int budget, const int recent) {
+  constexpr int WAVES = CHOOSERS / 64, PART = PER * CHOOSERS;
+  __shared__ int hist[BINS];
+  __shared__ unsigned ends[2][WAVES], few[FEW];
+  __shared__ int sums[WAVES], found[3], listed;
+  __shared__ int counts[2][PER * WAVES];
   const int seq = blockIdx.x, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
   const int len = max(0, min(seq_lens[seq], width * PAGE));
@@ -70,84 +106,197 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
   for (int i = tid; i < recent; i += CHOOSERS) out[heavy + i] = old + i;
   if (heavy == 0) return;
 
-  // ---- `left` of those that start with `prefix` stay
-  unsigned prefix = 0;
-  int left = heavy;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int i = tid; i < old; i += CHOOSERS) {
-      const unsigned x = w[i];
-      if ((x & mask) == prefix) atomicAdd(&hist[x >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (wave == 0) {                // digits from the top, four per lane
-      int n[4], mine = 0;
+  unsigned x[PER];                  // keys base + j * CHOOSERS + tid
+  auto load = [&](const int base) {
+    if constexpr (SUMS) {
+      const int* bt = block_tables + (int64_t)seq * width;
+      const float* at[PER];
+      double sum[PER];
 #pragma unroll
-      for (int j = 0; j < 4; j++) mine += n[j] = hist[255 - lane * 4 - j];
-      int above = mine;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int x = __shfl_up(above, off, 64);
-        if (lane >= off) above += x;
+      for (int j = 0; j < PER; j++) {
+        const int i = min(base + j * CHOOSERS + tid, old - 1);
+        at[j] = key_weights + (int64_t)bt[i / PAGE] * KH * PAGE + i % PAGE;
+        sum[j] = 0.;
       }
-      above -= mine;
+#pragma unroll 4
+      for (int h = 0; h < KH; h++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (above < left && above + n[j] >= left) {
-          found[0] = 255 - lane * 4 - j;
-          found[1] = left - above;
-        }
-        above += n[j];
+        for (int j = 0; j < PER; j++) sum[j] += (double)at[j][h * PAGE];
+#pragma unroll
+      for (int j = 0; j < PER; j++) x[j] = ordered((float)sum[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const int i = base + j * CHOOSERS + tid;
+        x[j] = i < old ? w[i] : 0u;
       }
     }
-    __syncthreads();
-    prefix |= (unsigned)found[0] << shift;
-    left = found[1];
-    __syncthreads();
+  };
+  auto parts = [&](auto each) {     // every part, read again unless it is the only one
+    for (int base = 0; base < (ONE ? 1 : old); base += PART) {
+      if (!ONE) load(base);
+      each(base);
+    }
+  };
+  if (ONE) load(0);
+
+  // ---- smallest and largest total
+  unsigned lo = ~0u, hi = 0u;
+  parts([&](const int base) {
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+      if (base + j * CHOOSERS + tid < old) {
+        lo = min(lo, x[j]);
+        hi = max(hi, x[j]);
+      }
+  });
+  hi = lanes_up_to(hi, Larger{});
+  lo = ~lanes_up_to(~lo, Larger{});
+  if (lane == 63) { ends[0][wave] = lo; ends[1][wave] = hi; }
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < WAVES; v++) {
+    lo = v ? min(lo, ends[0][v]) : ends[0][0];
+    hi = v ? max(hi, ends[1][v]) : ends[1][0];
   }
 
-  // ---- those above `prefix` and the first `left` equal ones, in order
-  int at = 0, ties = 0;             // kept and equal ones before this tile
-  const unsigned long long below = (1ull << lane) - 1;
-  for (int base = 0; base < old; base += CHOOSERS) {
-    const int i = base + tid;
-    const unsigned x = i < old ? w[i] : 0u;
-    const bool tie = i < old && x == prefix, more = i < old && x > prefix;
-    const unsigned long long t = __ballot(tie), m = __ballot(more);
-    if (lane == 0) {
-      counts[0][wave] = __popcll(t);
-      counts[1][wave] = __popcll(m);
+  // ---- `left` of the `some` in lo..hi stay, and all above hi
+  int left = heavy, some = old;
+  while (lo != hi && left != some && some > FEW) {  // uniform
+    // every turn leaves 2^-11 of the range
+    const int shift = max(0, 32 - __builtin_clz(hi - lo) - 11);
+    *reinterpret_cast<int2*>(hist + 2 * tid) = {0, 0};
+    __syncthreads();
+    parts([&](const int base) {
+      // A wave's equal totals would queue for one bin. Where its first row has many,
+      // those of the first lane's bin are one addition.
+      const int first = (x[0] - lo) >> shift;
+      const bool alike = __popcll(__ballot(
+          first == __builtin_amdgcn_readfirstlane(first))) > 16;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const unsigned d = x[j] - lo;
+        if (d > hi - lo || base + j * CHOOSERS + tid >= old) continue;
+        const int bin = d >> shift;
+        if (!alike) {
+          atomicAdd(&hist[bin], 1);
+          continue;
+        }
+        const int one = __builtin_amdgcn_readfirstlane(bin);
+        const unsigned long long same = __ballot(bin == one);
+        if (bin != one) atomicAdd(&hist[bin], 1);
+        else if (lanes_below(same) == 0) atomicAdd(&hist[bin], __popcll(same));
+      }
+    });
+    __syncthreads();
+    // two bins per thread, from the top
+    const int2 n = *reinterpret_cast<const int2*>(hist + BINS - 2 - 2 * tid);
+    int above = lanes_up_to(n.x + n.y, Plus{});
+    if (lane == 63) sums[wave] = above;
+    __syncthreads();
+    above -= n.x + n.y;
+#pragma unroll
+    for (int v = 0; v < WAVES; v++) above += v < wave ? sums[v] : 0;
+    const bool upper = above + n.y >= left;
+    if (above < left && above + n.x + n.y >= left) {
+      found[0] = BINS - 1 - 2 * tid - !upper;
+      found[1] = left - above - (upper ? 0 : n.y);
+      found[2] = upper ? n.y : n.x;
     }
     __syncthreads();
-    int t0 = ties, m0 = at, ts = 0, ms = 0;
-    for (int v = 0; v < WAVES; v++) {
-      if (v == wave) { t0 += ts; m0 += ms; }
-      ts += counts[0][v];
-      ms += counts[1][v];
-    }
-    // places before this key: those above, and the equal ones that stay
-    const int tie_rank = t0 + __popcll(t & below);
-    if (more || (tie && tie_rank < left))
-      out[m0 + __popcll(m & below) + min(tie_rank, left)] = i;
-    ties += ts;
-    at += ms;
-    __syncthreads();
+    lo += (unsigned)found[0] << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1);      // which may end at ~0
+    left = found[1];
+    some = found[2];
   }
+  if (lo != hi && left != some) {   // few: a wave ranks them, equal ones alike
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    parts([&](const int base) {
+#pragma unroll
+      for (int j = 0; j < PER; j++)
+        if (base + j * CHOOSERS + tid < old && x[j] >= lo && x[j] <= hi)
+          few[atomicAdd(&listed, 1)] = x[j];
+    });
+    __syncthreads();
+    if (wave == 0) {
+      const unsigned mine = lane < some ? few[lane] : 0u;
+      int more = 0, same = 0;
+#pragma unroll
+      for (int o = 0; o < FEW; o++) {
+        const unsigned y = __builtin_amdgcn_readlane(mine, o);
+        more += o < some && y > mine;
+        same += o < some && y == mine;
+      }
+      if (lane < some && more < left && more + same >= left) {
+        found[0] = (int)mine;       // the same from every lane that holds it
+        found[1] = left - more;
+      }
+    }
+    __syncthreads();
+    lo = hi = (unsigned)found[0];
+    left = found[1];
+  }
+
+  // ---- those above hi and the first `left` of the others, in order
+  int at = 0, ties = 0;             // kept and equal ones before this part
+  __syncthreads();
+  parts([&](const int base) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const bool in = base + j * CHOOSERS + tid < old;
+      const int t = __popcll(__ballot(in && x[j] - lo <= hi - lo));
+      const int m = __popcll(__ballot(in && x[j] > hi));
+      if (lane == 0) {
+        counts[0][j * WAVES + wave] = t;
+        counts[1][j * WAVES + wave] = m;
+      }
+    }
+    __syncthreads();
+    if (wave < 2) {                 // running sums, in the order of the keys
+      int* c = counts[wave];
+      int before = 0;
+#pragma unroll
+      for (int k = 0; k < PER * WAVES; k += 64) {
+        const int n = k + lane < PER * WAVES ? c[k + lane] : 0;
+        const int sum = lanes_up_to(n, Plus{});
+        if (k + lane < PER * WAVES) c[k + lane] = before + sum - n;
+        before += __builtin_amdgcn_readlane(sum, 63);
+      }
+      if (lane == 0) found[wave] = before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int i = base + j * CHOOSERS + tid;
+      const bool tie = i < old && x[j] - lo <= hi - lo;
+      const bool more = i < old && x[j] > hi;
+      const int rank = ties + counts[0][j * WAVES + wave] +
+          lanes_below(__ballot(tie));
+      const int m = at + counts[1][j * WAVES + wave] +
+          lanes_below(__ballot(more));
+      if (more || (tie && rank < left)) out[m + min(rank, left)] = i;
+    }
+    ties += found[0];
+    at += found[1];
+    __syncthreads();
+  });
 }
 
 constexpr int MOVERS = 256;
+constexpr int DEEP = 8;             // loads of a thread under way at once
 
-// ROW: bytes of a key in K and V. Arrays of a (sequence, kv head): K, V, weights.
-template <int ROW>
+// Columns of K, V (CHUNKS x 16 bytes, `parts` of them make a row) or the weights
+// of a (sequence, kv head).
+template <int CHUNKS>
 __global__ __launch_bounds__(MOVERS)
 void compact_kernel(uint8_t* __restrict__ k, uint8_t* __restrict__ v,
                     float* __restrict__ key_weights,
                     const int* __restrict__ block_tables,
                     const int* __restrict__ kept,
                     const int* __restrict__ kept_lens, const int width,
-                    const int places, const int pages, const int KH) {
+                    const int places, const int pages, const int KH,
+                    const int parts) {
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int seq = blockIdx.y, kvh = blockIdx.x % KH, which = blockIdx.x / KH;
   const int n = min(kept_lens[seq], min(places, width * PAGE));
@@ -160,22 +309,43 @@ void compact_kernel(uint8_t* __restrict__ k, uint8_t* __restrict__ v,
     if (page < 0 || page >= pages) return -1;
     return ((int64_t)page * KH + kvh) * PAGE + key % PAGE;
   };
-  auto walk = [&](auto* base, const int chunks) {
-    const int step = MOVERS / chunks;
-    for (int i0 = 0; i0 < n; i0 += step) {
-      const int i = i0 + threadIdx.x / chunks, c = threadIdx.x % chunks;
-      const int src = i < n ? from[i] : i;
-      const int64_t of = src != i ? row_of(src) : -1;
-      std::remove_reference_t<decltype(*base)> x{};
-      if (of >= 0) x = base[of * chunks + c];
+  // rows of `stride` elements, of which this workgroup moves `chunks`
+  auto walk = [&](auto* base, const int chunks, const int stride) {
+    typedef std::remove_reference_t<decltype(*base)> T;
+    const int step = MOVERS / chunks, c = threadIdx.x % chunks;
+    for (int i0 = threadIdx.x / chunks; i0 - (int)threadIdx.x / chunks < n;
+         i0 += step * DEEP) {
+      T x[DEEP];
+      int64_t of[DEEP], to[DEEP];
+      int src[DEEP];
+#pragma unroll
+      for (int j = 0; j < DEEP; j++) {
+        const int i = i0 + j * step;
+        src[j] = i < n ? from[i] : i;
+      }
+#pragma unroll
+      for (int j = 0; j < DEEP; j++) {
+        const int i = i0 + j * step;
+        const bool moves = i < n && src[j] != i;
+        of[j] = moves ? row_of(src[j]) : -1;
+        to[j] = moves ? row_of(i) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < DEEP; j++)
+        if (of[j] >= 0) x[j] = base[of[j] * stride + c];
       __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): loads have arrived
       __syncthreads();
-      const int64_t to = of >= 0 ? row_of(i) : -1;
-      if (to >= 0) base[to * chunks + c] = x;
+#pragma unroll
+      for (int j = 0; j < DEEP; j++)
+        if (of[j] >= 0 && to[j] >= 0) base[to[j] * stride + c] = x[j];
     }
   };
-  if (which == 2) walk(key_weights, 1);
-  else walk((u32x4*)(which ? v : k), ROW / 16);
+  if (which == 2 * parts) {
+    walk(key_weights, 1, 1);
+  } else {
+    const int part = which >> 1;
+    walk((u32x4*)(which & 1 ? v : k) + part * CHUNKS, CHUNKS, parts * CHUNKS);
+  }
 }
 
 }  // namespace
@@ -196,17 +366,31 @@ void heavy_keys(at::Tensor kept, at::Tensor kept_lens, at::Tensor key_weights,
   const keys::Guard guard(key_weights.device());
   auto stream = at::hip::getCurrentHIPStream();
   const int64_t most = width * PAGE;
-  const at::Tensor totals = at::empty({B, most}, kept.options());
-  unsigned* w = (unsigned*)totals.data_ptr<int>();
-  if (most > budget)
+  const int KH = key_weights.size(1);
+  const float* weights = key_weights.data_ptr<float>();
+  const int *tables = block_tables.data_ptr<int>(), *lens = seq_lens.data_ptr<int>();
+  // as many registers as the table's keys need; short caches' totals without a
+  // launch of their own
+  const bool own = most <= 8 * CHOOSERS && KH <= 16;
+  at::Tensor totals;
+  unsigned* w = nullptr;
+  if (!own && most > budget) {
+    totals = at::empty({B, most}, kept.options());
+    w = (unsigned*)totals.data_ptr<int>();
     hipLaunchKernelGGL(key_total_kernel, dim3((most + 255) / 256, B), dim3(256),
-                       0, stream, w, key_weights.data_ptr<float>(),
-                       block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
-                       (int)width, (int)key_weights.size(1), (int)budget);
-  hipLaunchKernelGGL(choose_keys_kernel, dim3(B), dim3(CHOOSERS), 0, stream,
-                     kept.data_ptr<int>(), kept_lens.data_ptr<int>(), w,
-                     seq_lens.data_ptr<int>(), (int)width, (int)budget,
-                     (int)recent);
+                       0, stream, w, weights, tables, lens, (int)width, KH,
+                       (int)budget);
+  }
+  auto choose = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(B), dim3(CHOOSERS), 0, stream,
+                       kept.data_ptr<int>(), kept_lens.data_ptr<int>(), w,
+                       weights, tables, lens, (int)width, KH, (int)budget,
+                       (int)recent);
+  };
+  if (own && most <= 2 * CHOOSERS) choose(choose_keys_kernel<2, true, true>);
+  else if (own) choose(choose_keys_kernel<8, true, true>);
+  else if (most <= 32 * CHOOSERS) choose(choose_keys_kernel<32, true, false>);
+  else choose(choose_keys_kernel<32, false, false>);
 }
 
 void compact_pages(at::Tensor k_cache, at::Tensor v_cache,
@@ -226,17 +410,22 @@ void compact_pages(at::Tensor k_cache, at::Tensor v_cache,
   const keys::Guard guard(key_weights.device());
   auto stream = at::hip::getCurrentHIPStream();
   const int KH = k_cache.size(1);
-#define CP_ROW(R_)                                                            \
-  if (row == R_)                                                              \
-    hipLaunchKernelGGL((compact_kernel<R_>), dim3(3 * KH, B), dim3(MOVERS), 0, \
-                       stream, (uint8_t*)k_cache.data_ptr(),                  \
+  const int64_t chunks = row / 16;
+  // columns that a workgroup moves: as few as fill the chip, 64 bytes at least
+  int64_t own = chunks;
+  while (own > 4 && 2 * KH * B * (chunks / own) < 512) own /= 2;
+  const int64_t parts = chunks / own;
+#define CP_CHUNKS(C_)                                                         \
+  if (own == C_)                                                              \
+    hipLaunchKernelGGL((compact_kernel<C_>), dim3((2 * parts + 1) * KH, B),   \
+                       dim3(MOVERS), 0, stream, (uint8_t*)k_cache.data_ptr(), \
                        (uint8_t*)v_cache.data_ptr(),                          \
                        key_weights.data_ptr<float>(),                         \
                        block_tables.data_ptr<int>(), kept.data_ptr<int>(),    \
                        kept_lens.data_ptr<int>(), (int)block_tables.size(1),  \
-                       (int)kept.size(1), (int)k_cache.size(0), KH)
-  CP_ROW(64); CP_ROW(128); CP_ROW(256); CP_ROW(512);
-#undef CP_ROW
+                       (int)kept.size(1), (int)k_cache.size(0), KH, (int)parts)
+  CP_CHUNKS(4); CP_CHUNKS(8); CP_CHUNKS(16); CP_CHUNKS(32);
+#undef CP_CHUNKS
 }
 
 }  // namespace kaito
