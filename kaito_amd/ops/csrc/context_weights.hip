@@ -7,12 +7,22 @@
 //
 // The second pass keeps the keys and lets the rows go by, so that every key's sum
 // has one owner: no atomics, the same bits every time. A workgroup is 4 waves x 64
-// keys of a kv head. S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the wave's K
-// stays in registers as the first operand; query rows, flattened over the heads of
-// the group (row = position * G + head), come in tiles of 64 through LDS, one
-// tile ahead (swizzled as flash_prefill.h's K). A lane holds one row of a tile and
-// 16 keys of every 32, so that m and 1 / l are per-lane scalars and a weight is a
-// multiply-add, an exponential and a multiply-add into its key's sum.
+// keys (32 with 256 dims) of a kv head. S^T = K Q^T on v_mfma_f32_32x32x16_bf16:
+// the wave's K stays in registers as the first operand; query rows, flattened over
+// the heads of the group (row = position * G + head), come in tiles of 64 through
+// LDS with their m and 1 / l, two tiles ahead (swizzled as flash_prefill.h's K). A
+// lane holds one row of half a tile and 16 keys of every 32, so that m and 1 / l
+// are per-lane scalars and a weight is a multiply-add, an exponential and a
+// multiply-add into its key's sum.
+//
+// What bounds it: the matrix unit's power. With operands of random bits the chip
+// takes 33.6 ns for a product of 32 x 32 x 16 on a SIMD, twice the 16.3 ns that
+// constant operands take (1.0 PFLOP/s); 2048 rows of 32 heads over 16384 keys and 8
+// kv heads of 128 are 261 us of such products, and the pass takes 268, beside 566 of
+// flash_prefill.h's twice as many. One product after another and then all weights
+// 381 us; the loop without masks and addresses 315; products and weights in turns
+// 298; tiles of 64 rows and fragments four products ahead of their use 268. Eight
+// waves that share a tile: 278.
 #include "flash_prefill.h"
 #include "keys_common.h"
 #include <torch/library.h>
@@ -24,9 +34,11 @@ namespace {
 using flash::hbf16x8;
 using flash::f32x16;
 
-constexpr int WKEYS = 64;           // keys of a wave
-constexpr int KEYS = 4 * WKEYS;     // of a workgroup
-constexpr int ROWS = 64;            // query rows of a tile
+// 32-key tiles of a wave: with 256 dims two of them do not fit the registers
+template <int D> constexpr int tiles_of = D <= 128 ? 2 : 1;
+constexpr int NW = 4;               // waves of a workgroup
+template <int D> constexpr int keys_of = NW * 32 * tiles_of<D>;
+constexpr int ROWS = 64;            // query rows of a tile, two halves
 
 struct WeightArgs {
   const short* q;
@@ -38,19 +50,21 @@ struct WeightArgs {
   const int* block_tables;
   int64_t q_ts;
   int max_blocks, KH, G;
-  unsigned div_g;                   // ceil(2^32 / G): rows / G by a product's high half
   float c;                          // scale * log2 e
 };
 
-// row / G, exact below 2^26 rows for G up to 64
-KAITO_DEV int rows_over(const int row, const WeightArgs& a) {
-  return a.G == 1 ? row : (int)__umulhi((unsigned)row, a.div_g);
+// x, of which the compiler does not know that: what is made of it is made there and
+// not kept in registers from ahead of the loop
+KAITO_DEV int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(256, 2)
+__global__ __launch_bounds__(NW * 64, 2)
 void key_weight_kernel(const WeightArgs a) {
-  constexpr int KK = D / 16, CK = D / 8, COPIES = ROWS * CK / 256;
+  constexpr int TH = NW * 64, KK = D / 16, CK = D / 8, COPIES = ROWS * CK / TH;
+  constexpr int NT = tiles_of<D>, KEYS = keys_of<D>, WKEYS = KEYS / NW;
   const int seq = blockIdx.y;
   const int kvh = blockIdx.x % a.KH, key0 = blockIdx.x / a.KH * KEYS;
   const int tok0 = a.cu[seq], q_len = a.cu[seq + 1] - tok0;
@@ -62,13 +76,13 @@ void key_weight_kernel(const WeightArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  __shared__ __attribute__((aligned(128))) short lds[2][ROWS * D];
+  __shared__ __attribute__((aligned(128))) short lds[3][ROWS * D + NW * 4 * ROWS];
 
   // ---- this wave's keys
   const int wkey = key0 + wave * WKEYS;
-  hbf16x8 kf[2][KK];
+  hbf16x8 kf[NT][KK];
 #pragma unroll
-  for (int t = 0; t < 2; t++) {
+  for (int t = 0; t < NT; t++) {
     const int key = min(wkey + t * 32 + lr, kv_len - 1);
     const int64_t row =
         ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
@@ -88,68 +102,202 @@ void key_weight_kernel(const WeightArgs a) {
     }
   }
 
-  // ---- the rows that see one of the workgroup's keys
-  const int rows = q_len * a.G;
-  const int first = max(0, key0 - q_abs0) * a.G / ROWS * ROWS;
-  auto stage = [&](const int r0, short* buf) {
+  // ---- positions that see one of the workgroup's keys, POS of them a tile: a row's
+  // position in the tile and its head do not change. Rows behind the last whole
+  // position stand for it and weigh nothing.
+  const int pos_n = ROWS / a.G, real = pos_n * a.G;
+  const int first = max(0, key0 - q_abs0) / pos_n * pos_n;
+  uint32_t q_off[COPIES];           // of this thread's copies, behind the tile's base
 #pragma unroll
-    for (int j = 0; j < COPIES; j++) {
-      const int s = j * 256 + tid, row = s / CK;
-      const int R = min(r0 + row, rows - 1), pos = rows_over(R, a);
-      const short* p = a.q + (int64_t)(tok0 + pos) * a.q_ts +
-          (kvh * a.G + R - pos * a.G) * D + flash::swz_k<D>(row, s % CK) * 8;
-      flash::lds_copy16(p, buf + (j * 256 + wave * 64) * 8);
-    }
+  for (int j = 0; j < COPIES; j++) {
+    const int s = j * TH + tid, row = min(s / CK, real - 1);
+    q_off[j] = (uint32_t)(row / a.G) * (uint32_t)a.q_ts + row % a.G * D +
+        flash::swz_k<D>(s / CK, s % CK) * 8;
+  }
+  // every wave stages all pairs of (maximum, 1 / sum) for itself: a word a lane, twice
+  uint32_t st_off[2];
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int row = min(u * 32 + (lane >> 1), real - 1);
+    st_off[u] = (row / a.G * QH + row % a.G) * 2 + (lane & 1);
+  }
+  const short* q_base = a.q + (int64_t)(tok0 + first) * a.q_ts + kvh * a.G * D;
+  const float* st_base = reinterpret_cast<const float*>(
+      a.stats + (int64_t)(tok0 + first) * QH + kvh * a.G);
+  auto copy4 = [&](const float* src, short* dst) {
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) unsigned int*)src,
+        (__attribute__((address_space(3))) unsigned int*)dst, 4, 0, 0);
   };
-  f32x16 sum[2];
+  auto stage = [&](const int p0, const int b) {     // tiles in their order
+    short* buf = lds[b];
+    short* pairs = buf + ROWS * D + wave * 4 * ROWS;
+    if (p0 + pos_n <= q_len) {
 #pragma unroll
-  for (int t = 0; t < 2; t++)
+      for (int j = 0; j < COPIES; j++)
+        flash::lds_copy16(q_base + q_off[j], buf + (j * TH + wave * 64) * 8);
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        copy4(st_base + st_off[u], pairs + u * 128);
+    } else if (p0 < q_len) {        // the last: behind its last position that again
+      const int last = q_len - 1 - p0, me = fresh(tid);
+#pragma unroll
+      for (int j = 0; j < COPIES; j++) {
+        const int s = j * TH + me, row = min(s / CK, real - 1);
+        flash::lds_copy16(
+            q_base + (int64_t)min(row / a.G, last) * a.q_ts + row % a.G * D +
+                flash::swz_k<D>(s / CK, s % CK) * 8,
+            buf + (j * TH + wave * 64) * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int row = min(u * 32 + ((me & 63) >> 1), real - 1);
+        copy4(st_base + (min(row / a.G, last) * QH + row % a.G) * 2 + (me & 1),
+              pairs + u * 128);
+      }
+    }
+    q_base += pos_n * a.q_ts;
+    st_base += pos_n * QH * 2;
+  };
+  f32x16 sum[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int i = 0; i < 16; i++) sum[t][i] = 0.f;
 
-  stage(first, lds[0]);
+  // A turn: the next half's products beside this half's weights. The matrix unit
+  // works on its own once a product is issued, but two waves of a SIMD that both
+  // multiply and then both weigh wait for each other (measured: the sum of both
+  // times), so that every product is followed by its share of the weights: the last
+  // addition of one share, the exponentials of the next, the exponents of the one
+  // behind. The scheduler gathers the products otherwise. The first fragments of
+  // the half after that are read on the way.
+  constexpr int FEW = 4;
+  hbf16x8 head[FEW];
+  auto fragment = [&](const short* half, const int kk) {
+    return *reinterpret_cast<const hbf16x8*>(
+        half + lr * D + flash::swz_k<D>(lr, kk * 2 + h) * 8);
+  };
+  auto turn = [&](const short* half, const short* after, f32x16 (&next)[NT],
+                  const f32x16 (&s)[NT], const float2_t st) {
+    constexpr int GROUPS = NT * KK, EACH = 16 / KK;
+    float x[16 * NT];
+    auto exponents = [&](const int g) {
+#pragma unroll
+      for (int e = g * EACH; e < (g + 1) * EACH; e++)
+        x[e] = fmaf(s[e / 16][e % 16], a.c, -st[0]);
+    };
+    auto weights = [&](const int g) {
+#pragma unroll
+      for (int e = g * EACH; e < (g + 1) * EACH; e++)
+        sum[e / 16][e % 16] = fmaf(x[e], st[1], sum[e / 16][e % 16]);
+    };
+    hbf16x8 qf[KK + FEW];
+#pragma unroll
+    for (int kk = 0; kk < FEW; kk++) qf[kk] = head[kk];
+    exponents(0);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) next[t][i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int kk = g / NT, t = g % NT;
+      if (t == 0)
+        qf[kk + FEW] = kk + FEW < KK ? fragment(half, kk + FEW)
+                                     : fragment(after, kk + FEW - KK);
+      next[t] = flash::mfma32(kf[t][kk], qf[kk], next[t]);
+      if (g > 0) weights(g - 1);
+#pragma unroll
+      for (int e = g * EACH; e < (g + 1) * EACH; e++)
+        x[e] = __builtin_amdgcn_exp2f(x[e]);
+      if (g + 1 < GROUPS) exponents(g + 1);
+    }
+    weights(GROUPS - 1);
+#pragma unroll
+    for (int kk = 0; kk < FEW; kk++) head[kk] = qf[KK + kk];
+  };
+
+  // In the step of a tile the next one is there and the one after it under way.
+  int at = 0, p0 = first;           // place of the tile at p0 among the three
+  stage(p0, 0);
+  stage(p0 + pos_n, 1);
   __syncthreads();
-  int cur = 0;
-  for (int r0 = first; r0 < rows; r0 += ROWS) {
-    if (r0 + ROWS < rows) stage(r0 + ROWS, lds[cur ^ 1]);
+  auto pair = [&](const short* tile, const int row) {
+    float2_t st = __builtin_bit_cast(
+        float2_t, *reinterpret_cast<const short4_t*>(
+                      tile + ROWS * D + wave * 4 * ROWS + 4 * row));
+    if (row >= real) st[1] = 0.f;
+    return st;
+  };
+  auto ahead = [&] { stage(p0 + 2 * pos_n, at == 0 ? 2 : at - 1); };
+  auto onward = [&] {
+    __syncthreads();
+    at = at == 2 ? 0 : at + 1;
+    p0 += pos_n;
+  };
+  auto clear = [&](f32x16 (&s)[NT]) {
 #pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[t][i] = 0.f;
+  };
+  // A tile whose rows do not all see all of the wave's keys: scores are of key
+  // wkey + 32 t + 8 (i / 4) + 4 h + i % 4, rows see those up to their position.
+  auto edge = [&] {
+    ahead();
     for (int u = 0; u < 2; u++) {
-      const int row = u * 32 + lr, R = r0 + row;
-      const int pos = rows_over(min(R, rows - 1), a);
-      const float2 st = a.stats[(int64_t)(tok0 + pos) * QH + kvh * a.G +
-                                min(R, rows - 1) - pos * a.G];
-      f32x16 s[2];
+      const int row = u * 32 + lr;
+      const float2_t st = pair(lds[at], row);
+      f32x16 s[NT];
+      clear(s);
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[t][i] = 0.f;
+        for (int t = 0; t < NT; t++)
+          s[t] = flash::mfma32(kf[t][kk], fragment(lds[at] + u * 32 * D, kk),
+                               s[t]);
+      const int pos = p0 + min(row, real - 1) / a.G;
+      const int last = pos < q_len ? q_abs0 + pos - wkey - 4 * h : -1;
 #pragma unroll
-      for (int kk = 0; kk < KK; kk++) {
-        const hbf16x8 qf = *reinterpret_cast<const hbf16x8*>(
-            lds[cur] + row * D + flash::swz_k<D>(row, kk * 2 + h) * 8);
-#pragma unroll
-        for (int t = 0; t < 2; t++) s[t] = flash::mfma32(kf[t][kk], qf, s[t]);
-      }
-      // key wkey + 32 t + 8 (i / 4) + 4 h + i % 4 of this lane's row; the last
-      // key that it sees, relative to the lane's first
-      const int last = R < rows ? q_abs0 + pos - wkey - 4 * h : -1;
-#pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float p =
-              __builtin_amdgcn_exp2f(fmaf(s[t][i], a.c, -st.x)) * st.y;
-          if (t * 32 + 8 * (i / 4) + i % 4 <= last) sum[t][i] += p;
+          float x = fmaf(s[t][i], a.c, -st[0]);
+          if (t * 32 + 8 * (i / 4) + i % 4 > last) x = -INFINITY;
+          sum[t][i] = fmaf(__builtin_amdgcn_exp2f(x), st[1], sum[t][i]);
         }
     }
-    __syncthreads();
-    cur ^= 1;
+    onward();
+  };
+  while (p0 < q_len && q_abs0 + p0 < key0 + KEYS - 1) edge();
+  if (p0 + pos_n <= q_len) {
+    f32x16 s0[NT], s1[NT];
+    clear(s0);
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+        s0[t] = flash::mfma32(kf[t][kk], fragment(lds[at], kk), s0[t]);
+#pragma unroll
+    for (int kk = 0; kk < FEW; kk++) head[kk] = fragment(lds[at] + 32 * D, kk);
+    do {
+      const short *tile = lds[at], *next = lds[at == 2 ? 0 : at + 1];
+      const float2_t st0 = pair(tile, lr), st1 = pair(tile, 32 + lr);
+      ahead();
+      turn(tile + 32 * D, next, s1, s0, st0);
+      turn(next, next + 32 * D, s0, s1, st1);
+      onward();
+    } while (p0 + pos_n <= q_len);
   }
+  if (p0 < q_len) edge();
+  __syncthreads();
 
   // ---- over the lanes' rows, then one thread per key
   float* total = reinterpret_cast<float*>(&lds[0][0]);
 #pragma unroll
-  for (int t = 0; t < 2; t++)
+  for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const float x = group_reduce_sum<32>(sum[t][i]);
@@ -158,7 +306,7 @@ void key_weight_kernel(const WeightArgs a) {
     }
   __syncthreads();
   const int key = key0 + tid;
-  if (key < kv_len) {
+  if (tid < KEYS && key < kv_len) {
     float* w = a.key_weights +
         ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
         key % keys::PAGE;
@@ -186,7 +334,8 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
   a.QH = q.size(1);
   a.KH = k_cache.size(1);
   const int G = a.QH / a.KH, D = q.size(2);
-  TORCH_CHECK(G <= 64 && T * G < (1 << 26), "rows of a step: 2^26 at most");
+  TORCH_CHECK(G <= ROWS, "unsupported GQA group ", G);
+  TORCH_CHECK(q.stride(0) < (1 << 25), "q: rows 2^25 apart at most");
   if (ntiles == 0 || T == 0 || block_tables.size(1) == 0) return;
   const keys::Guard guard(q.device());
   const at::Tensor stats = at::empty({T, a.QH, 2}, q.options().dtype(at::kFloat));
@@ -220,12 +369,9 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
   w.max_blocks = a.max_blocks;
   w.KH = a.KH;
   w.G = G;
-  w.div_g = (unsigned)(((1ull << 32) + G - 1) / G);
   w.c = a.scale * flash::LOG2E;
 
   const dim3 grid(flash::grid_size(a, ntiles));
-  const int64_t blocks = ((int64_t)a.max_blocks * keys::PAGE + KEYS - 1) / KEYS;
-  const dim3 wgrid(blocks * a.KH, B);
   auto stream = at::hip::getCurrentHIPStream();
   auto launch = [&](auto d, auto fp8) {
     constexpr int D_ = decltype(d)::value;
@@ -234,8 +380,10 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
     hipLaunchKernelGGL((flash::flash_prefill_kernel<D_, D_, SRC, false, false,
                             false, D_, flash::kvt<D_, D_>(), 4, true>),
                        grid, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((key_weight_kernel<D_, F_>), wgrid, dim3(256), 0, stream,
-                       w);
+    constexpr int KEYS = keys_of<D_>;
+    const int64_t blocks = ((int64_t)a.max_blocks * keys::PAGE + KEYS - 1) / KEYS;
+    hipLaunchKernelGGL((key_weight_kernel<D_, F_>), dim3(blocks * a.KH, B),
+                       dim3(NW * 64), 0, stream, w);
   };
   auto by_type = [&](auto d) {
     if (k_cache.dtype() == at::kByte) launch(d, std::true_type{});
