@@ -60,6 +60,54 @@ KAITO_DEV int fresh(int x) {
   return x;
 }
 
+// 32 keys per tile, those behind the last in its place: lane lr's, 8 dims in 16
+template <int D, bool FP8>
+KAITO_DEV void load_keys(hbf16x8 (&kf)[tiles_of<D>][D / 16], const WeightArgs& a,
+                         const int* bt, const int key0, const int kv_len,
+                         const int kvh, const int lr, const int h) {
+#pragma unroll
+  for (int t = 0; t < tiles_of<D>; t++) {
+    const int key = min(key0 + t * 32 + lr, kv_len - 1);
+    const int64_t row =
+        ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
+        key % keys::PAGE;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; kk++) {
+      const int64_t at = row * D + kk * 16 + h * 8;
+      if constexpr (FP8) {
+        float f[8];
+        fp8x8_to_f32(*reinterpret_cast<const u8x8_t*>((const uint8_t*)a.k + at),
+                     f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) kf[t][kk][e] = (__bf16)f[e];
+      } else {
+        kf[t][kk] = *reinterpret_cast<const hbf16x8*>((const short*)a.k + at);
+      }
+    }
+  }
+}
+
+// the lanes' rows together: total[key] of a wave's keys
+template <int NT>
+KAITO_DEV void sum_rows(float* total, const f32x16 (&sum)[NT], const int lr,
+                        const int h) {
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float x = group_reduce_sum<32>(sum[t][i]);
+      if (lr == 0) total[t * 32 + 8 * (i / 4) + 4 * h + i % 4] = x;
+    }
+}
+
+KAITO_DEV void add_weight(const WeightArgs& a, const int* bt, const int kvh,
+                          const int key, const int q_abs0, const float x) {
+  float* w = a.key_weights +
+      ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
+      key % keys::PAGE;
+  *w = (key < q_abs0 ? *w : 0.f) + x;
+}
+
 template <int D, bool FP8>
 __global__ __launch_bounds__(NW * 64, 2)
 void key_weight_kernel(const WeightArgs a) {
@@ -81,26 +129,7 @@ void key_weight_kernel(const WeightArgs a) {
   // ---- this wave's keys
   const int wkey = key0 + wave * WKEYS;
   hbf16x8 kf[NT][KK];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int key = min(wkey + t * 32 + lr, kv_len - 1);
-    const int64_t row =
-        ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
-        key % keys::PAGE;
-#pragma unroll
-    for (int kk = 0; kk < KK; kk++) {
-      const int64_t at = row * D + kk * 16 + h * 8;
-      if constexpr (FP8) {
-        float f[8];
-        fp8x8_to_f32(*reinterpret_cast<const u8x8_t*>((const uint8_t*)a.k + at),
-                     f);
-#pragma unroll
-        for (int e = 0; e < 8; e++) kf[t][kk][e] = (__bf16)f[e];
-      } else {
-        kf[t][kk] = *reinterpret_cast<const hbf16x8*>((const short*)a.k + at);
-      }
-    }
-  }
+  load_keys<D, FP8>(kf, a, bt, wkey, kv_len, kvh, lr, h);
 
   // ---- positions that see one of the workgroup's keys, POS of them a tile: a row's
   // position in the tile and its head do not change. Rows behind the last whole
@@ -296,22 +325,132 @@ void key_weight_kernel(const WeightArgs a) {
 
   // ---- over the lanes' rows, then one thread per key
   float* total = reinterpret_cast<float*>(&lds[0][0]);
+  sum_rows<NT>(total + wave * WKEYS, sum, lr, h);
+  __syncthreads();
+  const int key = key0 + tid;
+  if (tid < KEYS && key < kv_len) add_weight(a, bt, kvh, key, q_abs0, total[tid]);
+}
+
+// The same for steps that the kernel above leaves most of the chip without work in:
+// 8 waves share 64 keys and take 32 rows each in turn, straight from memory and a
+// turn ahead; their sums meet in LDS. No tile waits for another wave.
+template <int D, bool FP8>
+__global__ __launch_bounds__(512, 2)
+void key_weight_few_kernel(const WeightArgs a) {
+  constexpr int KK = D / 16, NT = tiles_of<D>, WKEYS = 32 * NT;
+  const int seq = blockIdx.y;
+  const int kvh = blockIdx.x % a.KH, key0 = blockIdx.x / a.KH * WKEYS;
+  const int tok0 = a.cu[seq], q_len = a.cu[seq + 1] - tok0;
+  const int kv_len = min(a.kv_lens[seq], a.max_blocks * keys::PAGE);
+  if (key0 >= kv_len || q_len <= 0) return;
+  const int* bt = a.block_tables + (int64_t)seq * a.max_blocks;
+  const int QH = a.KH * a.G, q_abs0 = kv_len - q_len;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  __shared__ float total[8][WKEYS];
+
+  const int rows = q_len * a.G, first = max(0, key0 - q_abs0) * a.G + wave * 32;
+  hbf16x8 qf[KK];
+  float2 st = {0.f, 0.f};
+  int last = -1;
+  auto fetch = [&](const int r0) {  // this lane's row, the last one in its place
+    const int R = r0 + lr, in = min(R, rows - 1);
+    const int pos = in / a.G, head = kvh * a.G + in % a.G;
+    const short* p = a.q + (int64_t)(tok0 + pos) * a.q_ts + head * D + h * 8;
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+      qf[kk] = *reinterpret_cast<const hbf16x8*>(p + kk * 16);
+    st = a.stats[(int64_t)(tok0 + pos) * QH + head];
+    last = R < rows ? q_abs0 + pos - key0 - 4 * h : -1;
+  };
+  fetch(first);
+  hbf16x8 kf[NT][KK];
+  load_keys<D, FP8>(kf, a, bt, key0, kv_len, kvh, lr, h);
+
+  f32x16 sum[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float x = group_reduce_sum<32>(sum[t][i]);
-      if (lr == 0)
-        total[wave * WKEYS + t * 32 + 8 * (i / 4) + 4 * h + i % 4] = x;
-    }
+    for (int i = 0; i < 16; i++) sum[t][i] = 0.f;
+  for (int r0 = first; r0 < rows; r0 += 8 * 32) {
+    f32x16 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[t][i] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+        s[t] = flash::mfma32(kf[t][kk], qf[kk], s[t]);
+    const float2 now = st;
+    const int seen = last;
+    if (r0 + 8 * 32 < rows) fetch(r0 + 8 * 32);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        float x = fmaf(s[t][i], a.c, -now.x);
+        if (t * 32 + 8 * (i / 4) + i % 4 > seen) x = -INFINITY;
+        sum[t][i] = fmaf(__builtin_amdgcn_exp2f(x), now.y, sum[t][i]);
+      }
+  }
+  sum_rows<NT>(total[wave], sum, lr, h);
   __syncthreads();
   const int key = key0 + tid;
-  if (tid < KEYS && key < kv_len) {
-    float* w = a.key_weights +
-        ((int64_t)bt[key / keys::PAGE] * a.KH + kvh) * keys::PAGE +
-        key % keys::PAGE;
-    *w = (key < q_abs0 ? *w : 0.f) + total[tid];
+  if (tid < WKEYS && key < kv_len) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) all += total[w][tid];
+    add_weight(a, bt, kvh, key, q_abs0, all);
   }
+}
+
+// The shares' outputs of a row and head joined, and what makes weights of its
+// scores. WPR waves a row: many shares are read in as few waits as four waves need.
+// Lane s has share s's maximum and sum.
+template <int D, int WPR>
+__global__ __launch_bounds__(256)
+void join_kernel(short* __restrict__ out, float2* __restrict__ stats,
+                 const float2* __restrict__ parts, const float* __restrict__ part,
+                 const int splits, const int64_t rows) {
+  constexpr int EACH = D / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  __shared__ float sums[WPR == 1 ? 1 : WPR][D];
+  if (row >= rows) return;          // with WPR > 1 none
+  const float2 mine = parts[min(lane, splits - 1) * rows + row];
+  const float m = wave_reduce_max(mine.x);
+  // a share whose sum is 0 has left no output; one that is no number does count
+  const float e = lane < splits && mine.y != 0.f
+      ? __builtin_amdgcn_exp2f(mine.x - m) : 0.f;
+  const float inv = 1.f / fmaxf(wave_reduce_sum(e == 0.f ? 0.f : e * mine.y), 1e-30f);
+  float o[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; i++) o[i] = 0.f;
+#pragma unroll 8
+  for (int s = WPR == 1 ? 0 : wave; s < splits; s += WPR) {
+    const float w = __builtin_bit_cast(
+        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), s));
+    const float* p = part + (s * rows + row) * D + lane * EACH;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) o[i] = fmaf(w, w == 0.f ? 0.f : p[i], o[i]);
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int i = 0; i < EACH; i++) sums[wave][lane * EACH + i] = o[i];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 0; i < EACH; i++)
+#pragma unroll
+      for (int v = 1; v < WPR; v++) o[i] += sums[v][lane * EACH + i];
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; i++)
+    out[row * D + lane * EACH + i] = f32_to_bf16(o[i] * inv);
+  if (lane == 0) stats[row] = {m, inv};
 }
 
 }  // namespace
@@ -335,6 +474,7 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
   a.KH = k_cache.size(1);
   const int G = a.QH / a.KH, D = q.size(2);
   TORCH_CHECK(G <= ROWS, "unsupported GQA group ", G);
+  TORCH_CHECK(T < (1ll << 31), "q: too many rows");
   TORCH_CHECK(q.stride(0) < (1 << 25), "q: rows 2^25 apart at most");
   if (ntiles == 0 || T == 0 || block_tables.size(1) == 0) return;
   const keys::Guard guard(q.device());
@@ -371,7 +511,22 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
   w.G = G;
   w.c = a.scale * flash::LOG2E;
 
-  const dim3 grid(flash::grid_size(a, ntiles));
+  // Few workgroups share out the keys too: as many shares as make two workgroups of
+  // a CU, of four tiles of the table's keys at least.
+  const int64_t groups = flash::grid_size(a, ntiles);
+  const int64_t tiles = (int64_t)a.max_blocks * keys::PAGE / (D <= 128 ? 64 : 32);
+  a.splits = std::max<int64_t>(
+      1, std::min<int64_t>({512 / groups, tiles / 4, 64}));
+  a.rows = (int)T;
+  at::Tensor part, parts;
+  if (a.splits > 1) {
+    const auto f32 = q.options().dtype(at::kFloat);
+    part = at::empty({a.splits, T, a.QH, D}, f32);
+    parts = at::empty({a.splits, T, a.QH, 2}, f32);
+    a.part = part.data_ptr<float>();
+    a.stats = (float2*)parts.data_ptr<float>();
+  }
+  const dim3 grid(groups, a.splits);
   auto stream = at::hip::getCurrentHIPStream();
   auto launch = [&](auto d, auto fp8) {
     constexpr int D_ = decltype(d)::value;
@@ -380,10 +535,29 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
     hipLaunchKernelGGL((flash::flash_prefill_kernel<D_, D_, SRC, false, false,
                             false, D_, flash::kvt<D_, D_>(), 4, true>),
                        grid, dim3(256), 0, stream, a);
-    constexpr int KEYS = keys_of<D_>;
-    const int64_t blocks = ((int64_t)a.max_blocks * keys::PAGE + KEYS - 1) / KEYS;
-    hipLaunchKernelGGL((key_weight_kernel<D_, F_>), dim3(blocks * a.KH, B),
-                       dim3(NW * 64), 0, stream, w);
+    const int64_t rows = T * a.QH;
+    auto join = [&](auto kernel, const int64_t groups) {
+      hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, a.out,
+                         (float2*)stats.data_ptr<float>(), a.stats, a.part,
+                         a.splits, rows);
+    };
+    if (a.splits > 8) join(join_kernel<D_, 4>, rows);
+    else if (a.splits > 1) join(join_kernel<D_, 1>, (rows + 3) / 4);
+    constexpr int KEYS = keys_of<D_>, SHARED = 32 * tiles_of<D_>;
+    const int64_t held = (int64_t)a.max_blocks * keys::PAGE;
+    auto blocks = [&](const int keys) {
+      return dim3((held + keys - 1) / keys * a.KH, B);
+    };
+    // Both in us, 256 keys a workgroup (64 shared): 512 rows of 4 heads on 512 keys,
+    // 16 workgroups, 41.5 and 22.5; on 1024 64 and 31; 1024 on 2048 98 and 54; four
+    // of 512 on 1024, 128 workgroups, 42.4 and 45.3; 1024 on 5120, 160, 75 and 115;
+    // 16 on 16016 12.1 and 42.8.
+    if (blocks(KEYS).x * B < 96)
+      hipLaunchKernelGGL((key_weight_few_kernel<D_, F_>), blocks(SHARED),
+                         dim3(512), 0, stream, w);
+    else
+      hipLaunchKernelGGL((key_weight_kernel<D_, F_>), blocks(KEYS), dim3(NW * 64),
+                         0, stream, w);
   };
   auto by_type = [&](auto d) {
     if (k_cache.dtype() == at::kByte) launch(d, std::true_type{});

@@ -85,7 +85,12 @@ struct Args {
   int db_n;
   float temp_coef;
   int temp_every;
-  float2* stats;                    // STATS: [T, QH] maximum (log2 domain), 1 / sum
+  // STATS: [T, QH] maximum (log2 domain), 1 / sum; with `splits` > 1 workgroups over
+  // a share of the key tiles each, [splits, T, QH] maximum, sum and, in `part`, the
+  // outputs times the sum in f32
+  float2* stats;
+  float* part;
+  int splits, rows;                 // rows: T
 };
 
 // LDS serves 256 bytes per cycle, 16 lanes of a 16-byte read, 32 of an 8-byte
@@ -214,8 +219,10 @@ void flash_prefill_kernel(const Args a) {
   // finite from the start (a sink may be -inf) and masked scores are -inf, at
   // any scale: a tile in which a row sees nothing neither moves the maximum
   // nor weighs anything.
-  float m = a.sinks ? fmaxf(a.sinks[head] * LOG2E, -1e30f) : -1e30f;
-  float l = (a.sinks || SIG) && h == 0 ? 1.0f : 0.f;
+  const int split = STATS ? blockIdx.y : 0;     // a sink is with the first keys
+  const bool sink = a.sinks && (!STATS || split == 0);
+  float m = sink ? fmaxf(a.sinks[head] * LOG2E, -1e30f) : -1e30f;
+  float l = (sink || SIG) && h == 0 ? 1.0f : 0.f;
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++)
@@ -223,13 +230,24 @@ void flash_prefill_kernel(const Args a) {
     for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
 
   // ---- key tiles: those with kept first keys, then the visible range
-  const int kv_end = min(kv_len, q_abs0 + q0 + QP);
+  int kv_end = min(kv_len, q_abs0 + q0 + QP);
   const int vis0 = EXT && a.chunk > 0 ? ((q_abs0 + q0) / a.chunk) * a.chunk
       : (a.window > 0 ? q_abs0 + q0 - a.window + 1 : 0);
   const int kv_begin = vis0 > 0 ? vis0 / KVT * KVT : 0;
   const int first_end =
       EXT ? min((a.keep_first + KVT - 1) / KVT * KVT, kv_begin) : 0;
-  const int kv_first = first_end > 0 ? 0 : kv_begin;
+  int kv_first = first_end > 0 ? 0 : kv_begin;
+  if constexpr (STATS) {            // no window, no kept keys: all tiles from 0 on
+    const int share =
+        ((kv_end + KVT - 1) / KVT + a.splits - 1) / a.splits * KVT;
+    kv_first = split * share;
+    kv_end = min(kv_end, kv_first + share);
+    if (kv_first >= kv_end) {
+      if (h == 0 && qrow < q_len)
+        a.stats[((int64_t)split * a.rows + tok0 + qrow) * a.QH + head] = {m, l};
+      return;
+    }
+  }
   auto next_tile = [&](const int kv0) {
     return EXT && kv0 + KVT == first_end ? kv_begin : kv0 + KVT;
   };
@@ -586,8 +604,20 @@ void flash_prefill_kernel(const Args a) {
   l = SIG ? 1.0f : l + __shfl_xor(l, 32, 64);
   if (qrow >= q_len) return;
   float inv = 1.0f / fmaxf(l, 1e-30f);
-  if constexpr (STATS)
-    if (h == 0) a.stats[(int64_t)(tok0 + qrow) * a.QH + head] = {m, inv};
+  if constexpr (STATS) {
+    const int64_t at = ((int64_t)split * a.rows + tok0 + qrow) * a.QH + head;
+    if (h == 0) a.stats[at] = {m, a.splits > 1 ? l : inv};
+    if (a.splits > 1) {
+      float* orow = a.part + at * DV + 4 * h;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+          *reinterpret_cast<float4_t*>(orow + dt * 32 + 8 * b) = float4_t{
+              o[dt][b * 4], o[dt][b * 4 + 1], o[dt][b * 4 + 2], o[dt][b * 4 + 3]};
+      return;
+    }
+  }
   if (EXT && a.gate) {
     const float g =
         bf16_to_f32(a.gate[(int64_t)(tok0 + qrow) * a.gate_s0 + head]);

@@ -156,6 +156,17 @@ def test_chunk_over_many_keys():
     _run("cuda", (16, 2, 64), [1030], [3], fp8=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", [(8, 2, 64), (8, 2, 128), (7, 1, 128),
+                                    (2, 2, 256)])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_few_rows_over_many_keys(layout, sinks):
+    """Keys shared out over workgroups; shares that a sequence does not reach."""
+    _run("cuda", layout, [5, 1, 70, 0, 33], [5000, 0, 130, 900, 2049], fp8=sinks,
+         sinks=sinks, seed=7)
+    _run("cuda", layout, [3], [13], sinks=sinks, width=600)
+
+
 @pytest.mark.parametrize("dev", CPU_OR_GPU)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("fp8", [False, True])
