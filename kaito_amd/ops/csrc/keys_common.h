@@ -24,8 +24,9 @@ inline void check_weights(const at::Tensor& key_weights,
                           const at::Tensor& block_tables) {
   TORCH_CHECK(key_weights.is_cuda() && key_weights.dtype() == at::kFloat &&
               key_weights.is_contiguous() && key_weights.dim() == 3 &&
-              key_weights.size(2) == PAGE && key_weights.size(1) > 0,
-              "key_weights: contiguous f32 [pages, kv heads, 16]");
+              key_weights.size(2) == PAGE && key_weights.size(1) > 0 &&
+              (uintptr_t)key_weights.data_ptr() % 16 == 0,
+              "key_weights: contiguous f32 [pages, kv heads, 16] in 16 bytes");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) <= 65535 &&
               block_tables.size(1) <= (1 << 26),
               "block_tables: [sequences, pages]");

@@ -95,10 +95,10 @@ struct DecodeArgs {
   int64_t k_stride, v_stride;
   const float* cos_sin;             // [positions, D]
   const int64_t* slots;             // [T]
-  // KEEP: scores (log2 domain), and what makes weights of them
+  // KEEP: scores (log2 domain), and the weights to come of them
   float* scores;                    // [T, QH, score_stride]
   int64_t score_stride;             // a multiple of KT that holds the table's keys
-  float2* stats;                    // [T, QH] maximum, 1 / sum
+  float* key_weights;               // [NB, KH, BS]
 
   // KEEP writes per key: never more of them than the table holds
   template <bool BIASED, bool KEEP = false>
@@ -224,6 +224,40 @@ KAITO_DEV Spans spans_of(const int seq_len, const int window, const int nsplit,
   return p;
 }
 
+// KEEP: what four keys, of one page, receive from the heads of a group, given their
+// maxima and 1 / sums; the row's own key begins anew. Scores behind `len` are there,
+// weights are not touched. One thread per four keys and kv head.
+KAITO_DEV void add_key_weights(const DecodeArgs& a, const int64_t row,
+                               const int kvh, const int key, const int len,
+                               const float2* stats) {
+  const int page = a.block_tables[row * a.max_blocks + key / BS];
+  f32x4* w = reinterpret_cast<f32x4*>(
+      a.key_weights + ((int64_t)page * a.KH + kvh) * BS + key % BS);
+  const float* s = a.scores + (row * a.KH + kvh) * a.G * a.score_stride + key;
+  f32x4 sum = *w;
+  const f32x4 old = sum;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (key + i + 1 == len) sum[i] = 0.f;
+  auto add = [&](const int g) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(s + g * a.score_stride);
+    const float2 st = stats[g];
+#pragma unroll
+    for (int i = 0; i < 4; i++)     // what the attention gives no weight has none here
+      if (x[i] > -1e29f)
+        sum[i] += __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
+  };
+  int g = 0;
+  for (; g + 4 <= a.G; g += 4)      // four heads' scores under way at once
+#pragma unroll
+    for (int j = 0; j < 4; j++) add(g + j);
+  for (; g < a.G; g++) add(g);
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (key + i >= len) sum[i] = old[i];
+  *w = sum;
+}
+
 template <int D, bool FP8, int NW, bool SPLIT, bool BIASED, bool ROPE,
           bool KEEP = false>
 __global__ __launch_bounds__(NW * 64, NW <= 4 && D <= 128 ? 3 : 2)
@@ -240,6 +274,7 @@ void paged_decode_kernel(const DecodeArgs a) {
   };
   __shared__ __attribute__((aligned(128))) short lds_v[NW][KT * D];
   __shared__ float s_m[NW][16], s_l[NW][16];
+  __shared__ float2 s_keep[KEEP ? 16 : 1];
   // BIASED: penalties of a wave's tile, heads by keys
   constexpr int PH = BIASED ? D <= 128 ? 8 : 4 : 1;
   __shared__ __attribute__((aligned(16))) float s_pen[BIASED ? NW : 1][PH * KT];
@@ -581,23 +616,30 @@ void paged_decode_kernel(const DecodeArgs a) {
     } else {
       if (a.sinks) den += fold_weight<BIASED>(sink, gm);
       if constexpr (KEEP)
-        if (d == 0)
-          a.stats[(int64_t)seq * QH + head] = {gm, 1.f / fmaxf(den, 1e-20f)};
+        if (d == 0) s_keep[g] = {gm, 1.f / fmaxf(den, 1e-20f)};
       store_head<BIASED>(a, seq, QH, head, D, d, num, den);
     }
+  }
+  if constexpr (KEEP) {
+    if (partial) return;            // uniform
+    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0): scores are stored
+    __threadfence_block();
+    __syncthreads();
+    for (int key = threadIdx.x * 4; key < seq_len; key += NW * 256)
+      add_key_weights(a, seq, kvh, key, seq_len, s_keep);
   }
 }
 
 // One workgroup per (sequence, head) folds the splits that had keys, unless
 // the first had them all. A chain of loads, so a short one: lane s of every
 // wave has split s's weight.
-template <int D, bool BIASED, bool KEEP = false>
+template <int D, bool BIASED>
 __global__ __launch_bounds__(D)
 void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
   const int64_t row = blockIdx.x, rows = gridDim.x;
   if (BIASED && a.token_seq[row / QH] < 0) return;
   const int used =
-      spans_of(a.len<BIASED, KEEP>(row / QH), a.window, splits, WIDE).used;
+      spans_of(a.len<BIASED>(row / QH), a.window, splits, WIDE).used;
   if (used == 1) return;
   constexpr float NONE = BIASED ? -INFINITY : -1e30f;
   const int d = threadIdx.x, lane = d & 63;
@@ -613,8 +655,6 @@ void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
   const float e = lane < used ? fold_weight<BIASED>(m, gm) : 0.f;
   float den = wave_reduce_sum(e * l);
   if (a.sinks) den += fold_weight<BIASED>(sink, gm);
-  if constexpr (KEEP)
-    if (d == 0) a.stats[row] = {gm, 1.f / fmaxf(den, 1e-20f)};
   float num = 0.f;
 #pragma unroll 4
   for (int s = 0; s < used; s++)
@@ -622,6 +662,56 @@ void paged_fold_kernel(const DecodeArgs a, const int QH, const int splits) {
                __builtin_bit_cast(int, e), s)) *
         a.part[(s * rows + row) * (D + 2) + d];
   store_head<BIASED>(a, row / QH, QH, (int)(row % QH), D, d, num, den);
+}
+
+// KEEP: the splits of a (sequence, kv head) are folded, and its keys' weights added,
+// by workgroups of 1024 keys each. All of them weigh the splits of all heads; the
+// heads' outputs are shared out among them.
+template <int D>
+__global__ __launch_bounds__(256)
+void paged_fold_weights_kernel(const DecodeArgs a, const int splits) {
+  __shared__ float s_e[16][64];
+  __shared__ float2 s_keep[16];
+  __shared__ float s_den[16];
+  const int64_t row = blockIdx.y, T = gridDim.y;
+  const int kvh = blockIdx.x % a.KH, chunk = blockIdx.x / a.KH;
+  const int QH = a.KH * a.G, len = a.len<false, true>(row);
+  const int used = spans_of(len, 0, splits, WIDE).used;
+  const int chunks = (len + 1023) / 1024;
+  if (used == 1 || chunk >= chunks) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto part = [&](const int s, const int g) {
+    return a.part + ((s * T + row) * QH + kvh * a.G + g) * (D + 2);
+  };
+  for (int g = wave; g < a.G; g += 4) {
+    const float sink = a.sinks ? a.sinks[kvh * a.G + g] * LOG2E : -1e30f;
+    float m = -1e30f, l = 0.f;
+    if (lane < used) {
+      m = part(lane, g)[D];
+      l = part(lane, g)[D + 1];
+    }
+    const float gm = fmaxf(wave_reduce_max(m), sink);
+    const float e = lane < used ? __builtin_amdgcn_exp2f(m - gm) : 0.f;
+    float den = wave_reduce_sum(e * l);
+    if (a.sinks) den += __builtin_amdgcn_exp2f(sink - gm);
+    s_e[g][lane] = e;
+    if (lane == 0) {
+      s_den[g] = den;
+      s_keep[g] = {gm, 1.f / fmaxf(den, 1e-20f)};
+    }
+  }
+  __syncthreads();
+  const int key = chunk * 1024 + threadIdx.x * 4;
+  if (key < len) add_key_weights(a, row, kvh, key, len, s_keep);
+  constexpr int HEADS = 256 / D;    // at once
+  for (int g0 = chunk * HEADS; g0 < a.G; g0 += chunks * HEADS) {
+    const int g = g0 + threadIdx.x / D, d = threadIdx.x % D;
+    if (g >= a.G) break;
+    float num = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < used; s++) num += s_e[g][s] * part(s, g)[d];
+    store_head<false>(a, row, QH, kvh * a.G + g, D, d, num, s_den[g]);
+  }
 }
 
 template <int D, bool FP8, bool BIASED, bool ROPE = false, bool KEEP = false>
@@ -662,8 +752,13 @@ void launch_paged_decode(DecodeArgs a, const at::Tensor& out, int T) {
                                 out.options().dtype(at::kFloat));
     a.part = part.data_ptr<float>();
     PA_LAUNCH(WIDE, true, dim3(pairs, splits));
-    hipLaunchKernelGGL((paged_fold_kernel<D, BIASED, KEEP>), dim3(T * a.KH * a.G),
-                       dim3(D), 0, stream, a, a.KH * a.G, (int)splits);
+    if constexpr (KEEP)
+      hipLaunchKernelGGL((paged_fold_weights_kernel<D>),
+                         dim3((a.max_blocks + 63) / 64 * a.KH, T), dim3(256), 0,
+                         stream, a, (int)splits);
+    else
+      hipLaunchKernelGGL((paged_fold_kernel<D, BIASED>), dim3(T * a.KH * a.G),
+                         dim3(D), 0, stream, a, a.KH * a.G, (int)splits);
   } else if (pairs <= (D <= 64 ? 512 : 256)) {
     PA_LAUNCH(WIDE, false, dim3(pairs));
   } else if ((pairs > ROUND2 / 2 && pairs <= ROUND2) ||
