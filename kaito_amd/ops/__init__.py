@@ -919,21 +919,19 @@ def context_attention(q: torch.Tensor, k_cache: torch.Tensor,
 
 
 # ---- a cache kept to a budget (kernel group "keys") -------------------------
+# GPU tensors are checked by the extension, CPU tensors here.
 
 def _own_pages(k_cache, v_cache, key_weights, block_tables) -> None:
-    """What the operators on weighted pages ask of them, on any device."""
     if k_cache.dim() != 4 or k_cache.size(2) != 16 \
             or v_cache.shape != k_cache.shape \
-            or v_cache.dtype != k_cache.dtype:
-        raise ValueError("k_cache and v_cache are [pages, kv heads, 16, "
-                         "head_dim] of one shape and type")
+            or v_cache.dtype != k_cache.dtype \
+            or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache and v_cache are contiguous [pages, kv heads,"
+                         " 16, head_dim] of one shape and type")
     _weighted_pages(key_weights, block_tables)
     if key_weights.shape != k_cache.shape[:3]:
         raise ValueError(f"key_weights {tuple(key_weights.shape)} do not "
                          f"belong to pages {tuple(k_cache.shape)}")
-    for t in (k_cache, v_cache):
-        if not t.is_contiguous():
-            raise ValueError("the caches have to be contiguous")
 
 
 def _weighted_pages(key_weights, block_tables) -> None:
@@ -945,24 +943,27 @@ def _weighted_pages(key_weights, block_tables) -> None:
         raise ValueError("block_tables is int32 [sequences, pages]")
 
 
-def _lengths_of(lens, block_tables, what: str) -> torch.Tensor:
-    if lens.dtype != torch.int32 or lens.dim() != 1 \
-            or lens.size(0) != block_tables.size(0):
-        raise ValueError(f"{what} is int32, one for each row of block_tables")
-    return lens.contiguous()
+def _per_row(t, n: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.shape != (n,):
+        raise ValueError(f"{what}: int32, {n} of them")
 
 
-def _query_rows(q, k_cache) -> torch.Tensor:
-    """q as the kernels read it: heads one behind another, rows in 16 bytes."""
+def _of_pages(q, k_cache) -> None:
     if q.dim() != 3 or q.size(2) != k_cache.size(3) \
             or q.size(1) % k_cache.size(1):
         raise ValueError(f"q {tuple(q.shape)} does not belong to pages "
                          f"{tuple(k_cache.shape)}")
-    D = q.size(2)
-    whole = q.stride(2) == 1 and q.stride(1) == D \
-        and (q.size(0) < 2 or q.stride(0) % 8 == 0) \
+
+
+def _query_rows(q) -> torch.Tensor:
+    """q as the kernels read it: heads one behind another, rows in 16 bytes."""
+    if q.dim() != 3:
+        return q                    # refused behind this
+    T, _, D = q.shape
+    ts, hs, ds = q.stride()
+    whole = ds == 1 and hs == D and (T < 2 or ts % 8 == 0) \
         and q.data_ptr() % 16 == 0
-    return q if whole else q.contiguous()
+    return q if whole else q.clone(memory_format=torch.contiguous_format)
 
 
 def context_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
@@ -982,22 +983,20 @@ def context_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
     nothing. Pages are a sequence's own here: what becomes of the weights of one
     that two tables of a call share is not defined. q bf16 of any strides, head
     sizes 64, 128 and 256, bf16 or e4m3 pages of 16 keys."""
-    _own_pages(k_cache, v_cache, key_weights, block_tables)
-    kv_lens = _lengths_of(kv_lens, block_tables, "kv_lens")
-    if cu_seqlens_q.dtype != torch.int32 \
-            or cu_seqlens_q.shape != (block_tables.size(0) + 1,):
-        raise ValueError("cu_seqlens_q is int32, one more than block_tables' "
-                         "rows")
-    q = _query_rows(q, k_cache)
     if q.is_cuda:
+        q = _query_rows(q)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         cu = cu_seqlens_q.contiguous()
         tile_seq, tile_qbase = tiles or _build_tiles(cu)
         _K.context_attention_weights(
             out, q, k_cache, v_cache, key_weights, tile_seq, tile_qbase, cu,
-            kv_lens, block_tables.contiguous(), scale,
+            kv_lens.contiguous(), block_tables.contiguous(), scale,
             _sinks_arg(sinks, q.device))
         return out
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    _of_pages(q, k_cache)
+    _per_row(kv_lens, block_tables.size(0), "kv_lens")
+    _per_row(cu_seqlens_q, block_tables.size(0) + 1, "cu_seqlens_q")
     return torch_ref.context_attention_weights(
         q, k_cache, v_cache, key_weights, cu_seqlens_q, kv_lens, block_tables,
         scale, sinks)
@@ -1013,17 +1012,18 @@ def paged_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
     last of seq_lens and begins anew. Rows of no keys come out as zeros. The
     scores are kept in f32 in between: 64 bytes for each row, query head and
     page of the table's width."""
-    _own_pages(k_cache, v_cache, key_weights, block_tables)
-    seq_lens = _lengths_of(seq_lens, block_tables, "seq_lens")
-    if q.size(0) != block_tables.size(0):
-        raise ValueError("q has one row for each row of block_tables")
-    q = _query_rows(q, k_cache)
     if q.is_cuda:
+        q = _query_rows(q)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _K.paged_attention_weights(
             out, q, k_cache, v_cache, key_weights, block_tables.contiguous(),
-            seq_lens, scale, _sinks_arg(sinks, q.device))
+            seq_lens.contiguous(), scale, _sinks_arg(sinks, q.device))
         return out
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    _of_pages(q, k_cache)
+    _per_row(seq_lens, q.size(0), "seq_lens")
+    if q.size(0) != block_tables.size(0):
+        raise ValueError("q has one row for each row of block_tables")
     return torch_ref.paged_attention_weights(
         q, k_cache, v_cache, key_weights, block_tables, seq_lens, scale, sinks)
 
@@ -1037,8 +1037,6 @@ def heavy_keys(key_weights: torch.Tensor, block_tables: torch.Tensor,
     [sequences, budget] int32, their places in ascending order, -1 behind the
     last; how many they are [sequences] int32). A sequence of up to `budget`
     keys keeps them all."""
-    _weighted_pages(key_weights, block_tables)
-    seq_lens = _lengths_of(seq_lens, block_tables, "seq_lens")
     if not 0 <= recent <= budget or budget < 1:
         raise ValueError(f"a budget of {budget} keys cannot hold the newest "
                          f"{recent}")
@@ -1049,8 +1047,10 @@ def heavy_keys(key_weights: torch.Tensor, block_tables: torch.Tensor,
         kept_lens = torch.empty(B, dtype=torch.int32,
                                 device=key_weights.device)
         _K.heavy_keys(kept, kept_lens, key_weights, block_tables.contiguous(),
-                      seq_lens, budget, recent)
+                      seq_lens.contiguous(), budget, recent)
         return kept, kept_lens
+    _weighted_pages(key_weights, block_tables)
+    _per_row(seq_lens, block_tables.size(0), "seq_lens")
     return torch_ref.heavy_keys(key_weights, block_tables, seq_lens, budget,
                                 recent)
 
@@ -1063,16 +1063,16 @@ def compact_pages(k_cache: torch.Tensor, v_cache: torch.Tensor,
     `kept` ascends; places at and behind kept_lens[b] stay as they were, and
     the pages behind it can be given back. Pages are a sequence's own: no page
     may be in two tables."""
-    _own_pages(k_cache, v_cache, key_weights, block_tables)
-    kept_lens = _lengths_of(kept_lens, block_tables, "kept_lens")
-    if kept.dtype != torch.int32 or kept.dim() != 2 \
-            or kept.size(0) != block_tables.size(0):
-        raise ValueError("kept is int32 [sequences, places]")
     if k_cache.is_cuda:
         _K.compact_pages(k_cache, v_cache, key_weights,
                          block_tables.contiguous(), kept.contiguous(),
-                         kept_lens)
+                         kept_lens.contiguous())
         return
+    _own_pages(k_cache, v_cache, key_weights, block_tables)
+    _per_row(kept_lens, block_tables.size(0), "kept_lens")
+    if kept.dtype != torch.int32 or kept.dim() != 2 \
+            or kept.size(0) != block_tables.size(0):
+        raise ValueError("kept is int32 [sequences, places]")
     torch_ref.compact_pages(k_cache, v_cache, key_weights, block_tables, kept,
                             kept_lens)
 

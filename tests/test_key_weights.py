@@ -361,3 +361,207 @@ def test_refusals(dev):
         refused(token, q, k, v, w, t, n, 1.0, torch.zeros(3, device=dev))
         refused(ops.heavy_keys, w, t, n.cpu(), 8, 0)
         refused(ops.compact_pages, k, k, w, t, kept, n)
+
+
+@pytest.mark.gpu
+def test_pages_far_behind():
+    """Pages whose rows lie beyond 2^31 elements of the caches."""
+    KH, D, far = 8, 128, 139000
+    k, v = (torch.empty(far + 40, KH, PAGE, D, dtype=torch.bfloat16,
+                        device="cuda") for _ in range(2))
+    w = torch.empty(far + 40, KH, PAGE, device="cuda")
+    small = _pages([300, 80], KH, D, width=19)
+    pages = torch.arange(far, far + small[0].size(0))
+    for x, y in zip((k, v, w), small):
+        x[pages.cuda()] = y.cuda()
+    tables = (small[3].long() + far).int().cuda()
+    lens = torch.tensor([300, 80], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 16, D).bfloat16().cuda()
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    want, near, want_w, off = _oracle(q, *small[:3], [1, 1], [300, 80], small[3],
+                                      D ** -0.5, None)
+    for op in ("paged", "context"):
+        w[pages.cuda()] = small[2].cuda()
+        out = ops.paged_attention_weights(q, k, v, w, tables, lens, D ** -0.5) \
+            if op == "paged" else ops.context_attention_weights(
+                q, k, v, w, cu, lens, tables, D ** -0.5)
+        err = (out.cpu().double() - want).abs()
+        assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20).all()
+        got = w[pages.cuda()].cpu().double()
+        assert ((got - want_w).abs() <= off)[off > 0].all()
+    kept, n = ops.heavy_keys(w, tables, lens, 64, 16)
+    assert torch.equal(kept.cpu(), _heavy(got.float(), small[3], [300, 80], 64, 16))
+    ops.compact_pages(k, v, w, tables, kept, n)
+    ref = [t.clone() for t in small[:2]] + [got.float()]
+    _close(*ref, small[3], kept.cpu(), n.tolist())
+    for x, y in zip((k, v, w), ref):
+        x = x[pages.cuda()].cpu()
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def _append(k, v, tables, lens, rows_k, rows_v):
+    """One new key a sequence, behind its last."""
+    b = torch.arange(len(lens), device=k.device)
+    page = tables[b, lens.long() // PAGE].long()
+    k[page, :, lens.long() % PAGE] = rows_k
+    v[page, :, lens.long() % PAGE] = rows_v
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+def test_a_cache_kept_to_its_budget(dev):
+    """Two prompts in chunks, then tokens, their caches cut every eight of them:
+    every output and all weights against 64 bits over the keys that are left."""
+    QH, KH, D, budget, recent = 4, 2, 64, 48, 16
+    scale = D ** -0.5
+    g = torch.Generator().manual_seed(2)
+    tables = torch.randperm(16, generator=g).int().view(2, 8)
+    # weights of rows that no one has written: a new key's must not count
+    k, v = (torch.full((16, KH, PAGE, D), math.nan).bfloat16() for _ in range(2))
+    w = torch.full((16, KH, PAGE), math.nan)
+    k, v, w, tables = (t.to(dev) for t in (k, v, w, tables))
+    lens = torch.zeros(2, dtype=torch.int32, device=dev)
+
+    def step(new):
+        """`new` rows of each sequence through the operator and the oracle."""
+        nonlocal lens
+        T = sum(new)
+        q, rk, rv = (torch.randn(T, n, D, generator=g).bfloat16().to(dev)
+                     for n in (QH, KH, KH))
+        at = 0
+        for b, n in enumerate(new):
+            for i in range(n):
+                _append(k, v, tables[b:b + 1], lens[b:b + 1] + i, rk[at:at + 1],
+                        rv[at:at + 1])
+                at += 1
+        lens = lens + torch.tensor(new, dtype=torch.int32, device=dev)
+        want, near, want_w, off = _oracle(q, k, v, w, new, lens.tolist(),
+                                          tables, scale, None)
+        if max(new) == 1:
+            out = ops.paged_attention_weights(q, k, v, w, tables, lens, scale)
+        else:
+            cu = torch.tensor([0] + new).cumsum(0).int().to(dev)
+            out = ops.context_attention_weights(q, k, v, w, cu, lens, tables,
+                                                scale)
+        err = (out.cpu().double() - want).abs()
+        assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20).all()
+        live = off > 0
+        assert ((w.cpu().double() - want_w).abs() <= off)[live].all()
+
+    step([40, 23])
+    step([30, 9])
+    for cut in range(3):
+        for _ in range(8):
+            step([1, 1])
+        kept, n = ops.heavy_keys(w, tables, lens, budget, recent)
+        want = _heavy(w.cpu(), tables.cpu(), lens.tolist(), budget, recent)
+        assert torch.equal(kept.cpu(), want)
+        ref = [t.cpu().clone() for t in (k, v, w)]
+        _close(*ref, tables.cpu(), want, n.tolist())
+        ops.compact_pages(k, v, w, tables, kept, n)
+        for x, y in zip((k, v, w), ref):
+            assert torch.equal(x.cpu().view(torch.uint8), y.view(torch.uint8))
+        lens = n
+        assert lens.tolist() == [48, min(48, 40 + 8 * cut)]
+
+
+@pytest.mark.gpu
+def test_replayed_from_graphs():
+    """Both attentions, the choice and the closing captured, two graphs of one
+    memory pool; eager work and other replays in between."""
+    KH, D = 2, 128
+    lens = [600, 33, 0, 2100]              # splits, and a padding row
+    k, v, w, tables = (t.cuda() for t in _pages(lens, KH, D, width=160, seed=4))
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    new = [3, 33, 0, 70]
+    cu = torch.tensor([0] + new).cumsum(0).int().cuda()
+    tiles = ops.build_query_tiles(new, "cuda")
+    q1 = torch.randn(4, 8, D).bfloat16().cuda()
+    q2 = torch.randn(106, 8, D).bfloat16().cuda()
+
+    def token(k, v, w):
+        return ops.paged_attention_weights(q1, k, v, w, tables, n, 0.1)
+
+    def cut(k, v, w):
+        out = ops.context_attention_weights(q2, k, v, w, cu, n, tables, 0.1,
+                                            tiles=tiles)
+        kept, left = ops.heavy_keys(w, tables, n, 500, 100)
+        ops.compact_pages(k, v, w, tables, kept, left)
+        return out, kept, left
+
+    eager = [t.clone() for t in (k, v, w)]
+    scratch = [t.clone() for t in eager]
+    token(*scratch), cut(*scratch)         # loaded before the capture
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        got1 = token(k, v, w)
+    with torch.cuda.graph(second, pool=first.pool()):
+        got2 = cut(k, v, w)
+    for t, e in zip((k, v, w), eager):
+        t.copy_(e)
+    for _ in range(4):
+        first.replay()
+        want = token(*eager)
+        assert torch.equal(got1, want)
+        torch.cuda.synchronize()
+        second.replay()
+        want = cut(*eager)
+        for a, b in zip(got2, want):
+            assert torch.equal(a, b)
+        for t, e in zip((k, v, w), eager):
+            assert torch.equal(t.view(torch.uint8), e.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_on_another_stream():
+    KH, D, lens = 2, 64, [1500, 40]
+    k, v, w, tables = (t.cuda() for t in _pages(lens, KH, D))
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    q = torch.randn(2, 8, D).bfloat16().cuda()
+
+    def run(k, v, w):
+        out = ops.paged_attention_weights(q, k, v, w, tables, n, 0.1)
+        kept, left = ops.heavy_keys(w, tables, n, 300, 20)
+        ops.compact_pages(k, v, w, tables, kept, left)
+        return out, kept, left
+
+    want_state = [t.clone() for t in (k, v, w)]
+    want = run(*want_state)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)      # the other stream is far ahead
+        got = run(k, v, w)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip([*got, k, v, w], [*want, *want_state]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_strided_arguments():
+    """Tables, lengths and choices cut from larger arrays; q of odd strides."""
+    KH, D, lens = 1, 64, [200, 90]
+    k, v, w, tables = (t.cuda() for t in _pages(lens, KH, D))
+    wide = torch.zeros(4, 30, dtype=torch.int32).cuda()
+    wide[::2, 3:3 + tables.size(1)] = tables
+    cut = wide[::2, 3:3 + tables.size(1)]
+    n = torch.tensor([200, 7, 90, 7], dtype=torch.int32).cuda()[::2]
+    x = torch.randn(2, 3 * D + 1, 2).bfloat16().cuda()
+    q = x[:, 1:1 + 2 * D].transpose(1, 2).reshape(2, 2, 2 * D)[:, :, ::2]
+    assert not cut.is_contiguous() and not n.is_contiguous()
+    a, b = w.clone(), w.clone()
+    assert torch.equal(
+        ops.paged_attention_weights(q, k, v, a, cut, n, 0.1),
+        ops.paged_attention_weights(q.contiguous(), k, v, b, tables,
+                                    n.contiguous(), 0.1))
+    assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+    kept, left = ops.heavy_keys(a, cut, n, 50, 5)
+    want = ops.heavy_keys(b, tables, n.contiguous(), 50, 5)
+    assert torch.equal(kept, want[0]) and torch.equal(left, want[1])
+    other = [t.clone() for t in (k, v, b)]
+    every = torch.full((2, 100), -7, dtype=torch.int32).cuda()
+    every[:, ::2] = kept
+    ops.compact_pages(k, v, a, cut, every[:, ::2], left)
+    ops.compact_pages(*other, tables, kept, left)
+    for s, t in zip((k, v, a), other):
+        assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
