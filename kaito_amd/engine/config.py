@@ -265,6 +265,14 @@ class EngineConfig:
     max_loras: int = 8
     max_lora_rank: int = 64
     enable_prefix_caching: bool = True      # block-hash APC (zero-copy)
+    # a bounded cache: once a sequence holds more than kv_budget +
+    # kv_budget_slack keys, every layer is cut to the kv_budget keys that
+    # have received the most attention, the newest kv_budget_recent always
+    # among them, and the pages behind are given back (None: all are kept).
+    # Keeps prefix caching, host offload and mixed steps off.
+    kv_budget: Optional[int] = None
+    kv_budget_recent: int = 256
+    kv_budget_slack: int = 128
     kv_offload: bool = False                # LMCache-style host KV cache
     kv_offload_bytes: Optional[int] = None  # None → 0.5 * available RAM
     # mixed steps: decode every step, with a bounded prefill chunk run

@@ -57,6 +57,11 @@ class LLMEngine:
             # stays off — the aliased (c, c) cache pair would double the
             # offloaded bytes in KVOffloadManager (models/mla.py)
             cfg.kv_offload = False
+        if cfg.kv_budget is not None:
+            self._check_budget(cfg)
+            # pages of a cut cache are its own, and hold no prefix
+            cfg.enable_prefix_caching = False
+            cfg.kv_offload = False
         self._maybe_enable_one_shot(cfg)
         self.runner = ModelRunner(cfg).load_model(weights_path, cfg.seed)
         self.runner.setup_tunable()
@@ -100,6 +105,60 @@ class LLMEngine:
         self.num_prompt_tokens = 0
         # optional KV event bus (EPP KVCache-aware routing surface)
         self.kv_publisher = None
+
+    @staticmethod
+    def _check_budget(cfg: EngineConfig) -> None:
+        from ..parallel.state import get_state
+        m, st = cfg.model, get_state()
+        group = m.num_heads // max(m.num_kv_heads, 1)
+        if not 0 <= cfg.kv_budget_recent <= cfg.kv_budget \
+                or cfg.kv_budget < 1 or cfg.kv_budget_slack < 0:
+            raise ValueError("kv_budget >= 1, 0 <= kv_budget_recent <= "
+                             "kv_budget and kv_budget_slack >= 0 are needed")
+        if m.is_mla or m.arch != "llama":
+            raise ValueError("kv_budget is for models whose attention layers "
+                             "keep rotary K and V pages")
+        if any(m.layer_sliding_window(i) for i in range(m.num_layers)):
+            raise ValueError("kv_budget: windows go by positions, which a cut "
+                             "cache does not keep")
+        if st.pp_size > 1 or cfg.enable_mixed_batch or cfg.block_size != 16:
+            raise ValueError("kv_budget needs pages of 16 keys, one pipeline "
+                             "stage and no mixed steps")
+        if str(cfg.device) != "cpu" and not (
+                m.head_dim == 128 and group <= 8
+                or m.head_dim == 64 and group in (1, 2, 4, 8)
+                or m.head_dim == 256 and group in (1, 2, 4)):
+            raise ValueError(f"kv_budget: no kernels for {group} heads of "
+                             f"{m.head_dim} per kv head")
+
+    def _cut_caches(self, seqs: List[Sequence]) -> None:
+        """Cuts the caches that have outgrown cfg.kv_budget, behind the step
+        just launched, and gives their pages back: whoever takes these comes
+        later in the same stream."""
+        cfg = self.cfg
+        if cfg.kv_budget is None:
+            return
+        cut, lens = [], []
+        for seq in seqs:
+            if not seq.block_table or seq.status == SeqStatus.FINISHED:
+                continue
+            keys = (seq.sched_len - 1 if seq.sched_len else
+                    seq.prefilled_len) - seq.evicted
+            if keys > cfg.kv_budget + cfg.kv_budget_slack:
+                cut.append(seq)
+                lens.append(keys)
+        if not cut:
+            return
+        self.runner.cut_caches([s.block_table for s in cut], lens,
+                               cfg.kv_budget, cfg.kv_budget_recent)
+        for seq, keys in zip(cut, lens):
+            seq.evicted += keys - cfg.kv_budget
+            need = self.pool.blocks_needed(seq.sched_tokens + 1 - seq.evicted)
+            free = seq.block_table[need:]
+            seq.block_table = seq.block_table[:need]
+            self.pool.free(free)
+            if self.kv_publisher is not None and free:
+                self.kv_publisher.block_removed(free)
 
     @staticmethod
     def _maybe_enable_one_shot(cfg: EngineConfig) -> None:
@@ -403,12 +462,14 @@ class LLMEngine:
             hidden = self.runner.execute_prefill(batch.chunks)
             samp = self._prefill_bookkeep(batch)
             if not samp:
+                self._cut_caches(batch.seqs)
                 return finished          # all chunks partial: no sampling
             tokens, lp = self._sample_prefill_pp(hidden, samp)
             finished += self._commit(samp, tokens.tolist(),
                                      [s.epoch for s in samp],
                                      self._lp_rows([lp + (0,)], len(samp))
                                      if lp is not None else None)
+            self._cut_caches(batch.seqs)
             return finished
 
         if self._pp:
@@ -451,6 +512,7 @@ class LLMEngine:
             event=event,
             index={s.seq_id: i for i, s in enumerate(batch.seqs)},
             lp_parts=[(lp_d[0], lp_d[1], 0)] if lp_d is not None else [])
+        self._cut_caches(batch.seqs)
         # resolve the PREVIOUS step while the GPU runs this one
         finished += self._resolve_pending()
         self._pending = new_pend

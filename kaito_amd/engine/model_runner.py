@@ -51,6 +51,8 @@ class ModelRunner:
             ops.load_extension(*groups)
         self.kv_caches: List[Tuple[torch.Tensor, torch.Tensor]] = []
         self.num_gpu_blocks = 0
+        # per layer, what the cached keys have received (cfg.kv_budget)
+        self.key_weights: Optional[List[torch.Tensor]] = None
         self.max_model_len = cfg.max_model_len or cfg.model.max_position
         self._graphs: Dict[int, tuple] = {}
         self._graph_pool = None
@@ -111,6 +113,8 @@ class ModelRunner:
         else:
             block_bytes = 2 * m.num_layers * kvh * cfg.block_size \
                 * m.head_dim * elem
+        if cfg.kv_budget is not None:
+            block_bytes += m.num_layers * kvh * cfg.block_size * 4
         if cfg.num_gpu_blocks is not None:
             n_blocks = cfg.num_gpu_blocks
         elif self.is_gpu:
@@ -143,6 +147,10 @@ class ModelRunner:
             v = torch.zeros_like(k)
             kvs.append((k, v))
         self.kv_caches = kvs
+        if cfg.kv_budget is not None:
+            self.key_weights = [
+                torch.zeros(n_blocks, kvh, cfg.block_size, device=self.device)
+                for _ in kvs]
         logger.info("KV pool: %d blocks (%d tokens), %.2f GiB", n_blocks,
                     n_blocks * cfg.block_size,
                     n_blocks * block_bytes / (1 << 30))
@@ -188,7 +196,7 @@ class ModelRunner:
         in chunk order (aligned with batch.sampling_seqs) — or, with
         `rows` (indices into the concatenated chunk rows), of exactly
         those rows."""
-        fresh = (not self.stateful
+        fresh = (not self.stateful and self.key_weights is None
                  and all(c.start == 0 and c.completes for c in chunks))
         dev, bs = self.device, self.cfg.block_size
         lens = np.array([c.length for c in chunks], dtype=np.int64)
@@ -209,6 +217,7 @@ class ModelRunner:
             p = np.arange(c.start, c.start + c.length)
             pos[a:b] = p
             table = np.array(c.seq.block_table, dtype=np.int64)
+            p = p - c.seq.evicted
             slots[a:b] = table[p // bs] * bs + p % bs
         wide = torch.from_numpy(wide).to(dev)
         input_ids, positions, slot_mapping = (
@@ -220,7 +229,8 @@ class ModelRunner:
             for i, c in enumerate(chunks):
                 flat[i, :len(c.seq.block_table)] = c.seq.block_table
             narrow["block_tables"] = flat
-            narrow["kv_lens"] = starts + lens
+            narrow["kv_lens"] = starts + lens - [c.seq.evicted
+                                                 for c in chunks]
         if self.stateful:
             narrow["state_slots"] = [c.seq.state_slot for c in chunks]
             narrow["seq_starts"] = starts
@@ -249,7 +259,8 @@ class ModelRunner:
             is_prefill=True, slot_mapping=slot_mapping,
             cu_seqlens=d["cu"], max_seqlen=max_seqlen,
             block_tables=d.get("block_tables"), kv_lens=d.get("kv_lens"),
-            tile_seq=d.get("tile_seq"), tile_qbase=d.get("tile_qbase"))
+            tile_seq=d.get("tile_seq"), tile_qbase=d.get("tile_qbase"),
+            key_weights=self.key_weights)
         if self.stateful:
             meta.state_slots = d["state_slots"]
             meta.seq_starts = d["seq_starts"]
@@ -275,7 +286,11 @@ class ModelRunner:
     def _init_decode_buffers(self):
         cfg = self.cfg
         max_bs = max(max(cfg.graph_batch_sizes), cfg.max_num_seqs)
-        mb = cfg.max_blocks_per_seq(self.max_model_len)
+        longest = self.max_model_len
+        if cfg.kv_budget is not None:   # caches are cut before they decode
+            longest = min(longest, cfg.kv_budget + cfg.kv_budget_slack
+                          + 2 * cfg.block_size)
+        mb = cfg.max_blocks_per_seq(longest)
         dev = self.device
         # the per-row inputs are rows of two blocks, so that a rebuilt batch
         # arrives in one copy each
@@ -330,7 +345,7 @@ class ModelRunner:
             is_prefill=False,
             slot_mapping=b["slot_mapping"][:bs],
             block_tables=b["block_tables"][:bs],
-            seq_lens=b["seq_lens"][:bs])
+            seq_lens=b["seq_lens"][:bs], key_weights=self.key_weights)
         if self.stateful:
             meta.cu_seqlens = b["cu_seqlens"][:bs + 1]
             meta.state_slots = b["state_slots"][:bs]
@@ -490,8 +505,9 @@ class ModelRunner:
                     b["block_tables"][i, :n].copy_(torch.tensor(
                         s.block_table, dtype=torch.int32), non_blocking=True)
                     s._bt_dirty = False
-            # slot = bt[i, pos // BS] * BS + pos % BS  (device-side gather)
-            pos = b["positions"][:bs]
+            # slot = bt[i, key // BS] * BS + key % BS  (device-side gather) of
+            # the row's own key, its cache's last
+            pos = b["seq_lens"][:bs].long() - 1
             blk = torch.gather(b["block_tables"][:bs].long(), 1,
                                (pos // self.cfg.block_size).unsqueeze(1)).squeeze(1)
             b["slot_mapping"][:bs].copy_(
@@ -504,6 +520,7 @@ class ModelRunner:
             narrow[1:3] = -1
             dst, src = [], []
             lens = [s.sched_tokens for s in seqs]
+            keys = np.array([n - s.evicted for n, s in zip(lens, seqs)])
             bsz = self.cfg.block_size
             flat = np.zeros((bs, self._max_blocks), dtype=np.int32)
             for i, s in enumerate(seqs):
@@ -515,12 +532,12 @@ class ModelRunner:
                     wide[0, i] = s.last_token_id
                 table = s.block_table
                 flat[i, :len(table)] = table
-                wide[2, i] = table[(lens[i] - 1) // bsz]
+                wide[2, i] = table[(keys[i] - 1) // bsz]
                 s._bt_dirty = False
-            narrow[0, :bs] = lens
-            pos = narrow[0, :bs].astype(np.int64) - 1
+            narrow[0, :bs] = keys
+            pos = np.array(lens, dtype=np.int64) - 1
             wide[1, :bs] = pos
-            wide[2, :bs] = wide[2, :bs] * bsz + pos % bsz
+            wide[2, :bs] = wide[2, :bs] * bsz + (keys - 1) % bsz
             if self.lora_manager is not None:
                 narrow[1, :bs] = [s.lora_id for s in seqs]
             if self.stateful:
@@ -543,6 +560,25 @@ class ModelRunner:
             g.replay()
             return out[:bs]
         return self._decode_forward(bs)
+
+    # ------------------------------------------------------------- budget
+    @torch.no_grad()
+    def cut_caches(self, tables: List[List[int]], lens: List[int],
+                   budget: int, recent: int) -> None:
+        """Cuts the caches of sequences (their pages, their keys) to `budget`
+        keys each, every layer by its own weights, in the current stream."""
+        from .. import ops
+        mb = max(len(t) for t in tables)
+        flat = np.zeros((len(tables), mb + 1), dtype=np.int32)
+        for i, t in enumerate(tables):
+            flat[i, :len(t)] = t
+        flat[:, mb] = lens
+        flat = torch.from_numpy(flat).to(self.device)
+        table, lens = flat[:, :mb].contiguous(), flat[:, mb].contiguous()
+        for (k, v), w in zip(self.kv_caches, self.key_weights):
+            kept, n = ops.heavy_keys(w, table, lens, budget, recent)
+            ops.compact_pages(k, v, w, table, kept, n)
+        self._last_ids = []             # the next decode step is built anew
 
     # ------------------------------------------------------------- step
     @torch.no_grad()

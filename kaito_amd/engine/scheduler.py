@@ -217,7 +217,8 @@ class Scheduler:
         i = 0
         while i < len(batch):
             seq = batch[i]
-            need = self.pool.blocks_needed(seq.sched_tokens + 1) - len(seq.block_table)
+            need = self.pool.blocks_needed(
+                seq.sched_tokens + 1 - seq.evicted) - len(seq.block_table)
             if need > 0:
                 if self.pool.can_allocate(need):
                     seq.block_table.extend(self.pool.allocate(need))
@@ -234,6 +235,7 @@ class Scheduler:
                     victim.block_table = []
                     victim.sched_len = 0
                     victim.prefilled_len = 0
+                    victim.evicted = 0
                     victim.epoch += 1
                     victim.status = SeqStatus.WAITING
                     self.waiting.appendleft(victim)

@@ -58,6 +58,9 @@ class Sequence:
     lora_id: int = -1            # adapter slot (-1 = base model)
     # recurrent-state slot (models with per-sequence state; -1 = none)
     state_slot: int = -1
+    # keys cut from the cache (EngineConfig.kv_budget): the token at position
+    # p is key p - evicted of it
+    evicted: int = 0
     # prompt tokens whose KV is in the cache (chunked prefill / prefix
     # restore); prompt fully prefilled when == num_prompt_tokens
     prefilled_len: int = 0

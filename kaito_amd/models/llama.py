@@ -52,6 +52,9 @@ class AttnMetadata:
     ctx_lens: Optional[list] = None
     # host copy of seq_starts, kept beside ctx_lens
     ctx_starts: Optional[list] = None
+    # per layer, what the cached keys have received (EngineConfig.kv_budget):
+    # [blocks, kv heads, block_size] f32, in place
+    key_weights: Optional[list] = None
     # values one layer of a step leaves for later layers of the same step
     # (the model's forward sets an empty dict)
     layer_shared: Optional[dict] = None
@@ -101,6 +104,7 @@ class LlamaAttention(nn.Module):
         super().__init__()
         tp = get_state().tp_size
         self.cfg = cfg
+        self.layer_idx = layer_idx
         self.head_dim = cfg.head_dim
         self.num_heads = cfg.num_heads // tp
         self.num_kv_heads = max(cfg.num_kv_heads // tp, 1)
@@ -165,6 +169,16 @@ class LlamaAttention(nn.Module):
         cs = cos_sin_local if self.local_rope else cos_sin
         T = qkv.size(0)
         sinks = getattr(self, "sinks", None)
+        weights = meta.key_weights[self.layer_idx] if meta.key_weights else None
+        if kv_cache is not None and not meta.is_prefill and weights is not None:
+            q, k = ops.rope_and_cache(positions, q, k, v, self.head_dim, cs,
+                                      kv_cache[0], kv_cache[1],
+                                      meta.slot_mapping)
+            out = ops.paged_attention_weights(
+                q.unflatten(-1, (self.num_heads, self.head_dim)), kv_cache[0],
+                kv_cache[1], weights, meta.block_tables, meta.seq_lens,
+                self.scale, sinks)
+            return o_proj(out.reshape(T, -1))
         if kv_cache is not None and not meta.is_prefill:
             out = ops.rope_paged_attention(
                 positions, q, k, v, self.head_dim, cs, kv_cache[0],
@@ -182,7 +196,11 @@ class LlamaAttention(nn.Module):
         vh = v.unflatten(-1, (self.num_kv_heads, self.head_dim))
         tiles = None if meta.tile_seq is None else \
             (meta.tile_seq, meta.tile_qbase)
-        if meta.kv_lens is not None:
+        if weights is not None:
+            out = ops.context_attention_weights(
+                qh, kv_cache[0], kv_cache[1], weights, meta.cu_seqlens,
+                meta.kv_lens, meta.block_tables, self.scale, sinks, tiles)
+        elif meta.kv_lens is not None:
             # suffix-query attention over the paged cache (the suffix
             # K/V was just written by rope_and_cache above)
             out = ops.context_attention(qh, kv_cache[0], kv_cache[1],

@@ -38,6 +38,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--swap-space", type=float, default=0.0,
                    help="GiB of host RAM for KV offload (LMCache analog)")
     p.add_argument("--kv-cache-dtype", default="auto")
+    p.add_argument("--kv-budget", type=int, default=None,
+                   help="keys that a sequence's cache keeps per layer: "
+                        "beyond them (and a slack of 128) those that have "
+                        "received the least attention are cut, the newest "
+                        "256 never (no prefix caching, no swap space)")
     p.add_argument("--enable-kv-events", action="store_true",
                    help="publish BlockStored/BlockRemoved on :5557 "
                         "(EPP KVCache-aware routing)")
@@ -136,6 +141,7 @@ def main(argv=None):
         kv_offload_bytes=int(args.swap_space * (1 << 30)) or None,
         kv_cache_dtype=("fp8" if args.kv_cache_dtype in
                         ("fp8", "fp8_e4m3") else "auto"),
+        kv_budget=args.kv_budget,
     )
     if args.kv_cache_dtype not in ("auto", "bf16", "bfloat16", "fp8",
                                    "fp8_e4m3"):

@@ -1,0 +1,190 @@
+"""Serving with caches kept to a budget (EngineConfig.kv_budget): the engine
+against a replay of the same model whose attention keeps plain lists of keys per
+sequence and layer, and cuts them by the rule, key by key."""
+import dataclasses
+
+import pytest
+import torch
+
+from kaito_amd import ops
+from kaito_amd.engine import EngineConfig, LLMEngine, SamplingParams
+from kaito_amd.models import get_model_config
+from kaito_amd.models.llama import AttnMetadata, LlamaAttention
+from kaito_amd.parallel.state import init_parallel
+
+SP = SamplingParams(max_tokens=60, ignore_eos=True)
+
+
+@pytest.fixture(autouse=True)
+def _parallel():
+    init_parallel(1)
+
+
+def _cfg(**kw):
+    base = dict(model=get_model_config("tiny-llama-test"), device="cpu",
+                max_num_seqs=8, num_gpu_blocks=64, enforce_eager=True,
+                max_model_len=256, kv_budget=32, kv_budget_recent=8,
+                kv_budget_slack=8)
+    base.update(kw)
+    return EngineConfig(**base)
+
+
+class _Lists:
+    """One sequence's keys, values and received weights, per layer."""
+
+    def __init__(self, cfg):
+        self.cfg, self.layers = cfg, {}
+
+    def attend(self, attn, qkv, positions, kv_cache, meta, cos_sin, *_):
+        q, k, v = qkv.split([attn.q_size, attn.kv_size, attn.kv_size], dim=-1)
+        q, k = ops.rotary_embedding(positions, q.clone(), k.clone(),
+                                    attn.head_dim, cos_sin)
+        D, T = attn.head_dim, qkv.size(0)
+        k, v = (t.reshape(T, attn.num_kv_heads, D) for t in (k, v))
+        if attn.layer_idx in self.layers:
+            K, V, W = self.layers[attn.layer_idx]
+            k, v = torch.cat([K, k]), torch.cat([V, v])
+            W = torch.cat([W, W.new_zeros(T, W.size(1))])
+        else:
+            W = torch.zeros(T, attn.num_kv_heads)
+        L, G = k.size(0), attn.num_heads // attn.num_kv_heads
+        x = q.reshape(T, attn.num_heads, D).float().transpose(0, 1)
+        kx, vx = (t.float().repeat_interleave(G, 1).transpose(0, 1)
+                  for t in (k, v))
+        s = x @ kx.transpose(1, 2) * attn.scale
+        later = torch.arange(L) > torch.arange(L - T, L)[:, None]
+        p = s.masked_fill(later, float("-inf")).softmax(-1)
+        W = W + p.unflatten(0, (-1, G)).sum((1, 2)).T
+        self.layers[attn.layer_idx] = (k, v, W)
+        out = (p @ vx).transpose(0, 1).to(qkv.dtype)
+        return attn.o_proj(out.reshape(T, -1))
+
+    def cut(self):
+        c = self.cfg
+        for i, (k, v, w) in self.layers.items():
+            L = k.size(0)
+            if L <= c.kv_budget + c.kv_budget_slack:
+                continue
+            total = w.double().sum(1).float()[:L - c.kv_budget_recent].tolist()
+            order = sorted(range(len(total)), key=lambda j: (-total[j], j))
+            stay = sorted(order[:c.kv_budget - c.kv_budget_recent]) \
+                + list(range(L - c.kv_budget_recent, L))
+            self.layers[i] = (k[stay], v[stay], w[stay])
+
+
+def _replayed(eng, prompt, n, monkeypatch, chunk=10 ** 9):
+    """n greedy tokens of a sequence by itself."""
+    lists, model = _Lists(eng.cfg), eng.runner.model
+    with monkeypatch.context() as m:
+        m.setattr(LlamaAttention, "attend",
+                  lambda attn, *a: lists.attend(attn, *a))
+        toks, at = list(prompt), 0
+        while len(toks) < len(prompt) + n:
+            end = min(at + chunk, len(toks))
+            ids = torch.tensor(toks[at:end])
+            T = end - at
+            meta = AttnMetadata(
+                is_prefill=True, slot_mapping=torch.full((T,), -1),
+                cu_seqlens=torch.tensor([0, T], dtype=torch.int32),
+                max_seqlen=T)
+            hidden = model(ids, torch.arange(at, end),
+                           [None] * model.num_local_layers, meta)
+            at = end
+            if at == len(toks):
+                toks.append(int(model.compute_logits(hidden[-1:]).argmax(-1)))
+            lists.cut()
+    return toks[len(prompt):]
+
+
+def test_a_budget_that_holds_everything_changes_nothing():
+    prompts = [list(range(5, 45)), [3, 5, 7]]
+    want = LLMEngine(_cfg(kv_budget=None)).generate(prompts, SP)
+    got = LLMEngine(_cfg(kv_budget=200)).generate(prompts, SP)
+    for a, b in zip(want, got):
+        assert a.output_token_ids == b.output_token_ids and b.evicted == 0
+
+
+@pytest.mark.parametrize("prompt", [[3, 14, 15], list(range(7, 39)),
+                                    list(range(10, 110))])
+def test_cut_caches_match_plain_lists(prompt, monkeypatch):
+    eng = LLMEngine(_cfg())
+    out = eng.generate([prompt], SP)[0]
+    assert out.evicted > 0
+    assert out.output_token_ids == _replayed(eng, prompt, 60, monkeypatch)
+    assert eng.pool.num_free == eng.pool.num_blocks
+
+
+def test_batches_chunks_and_joins(monkeypatch):
+    """Sequences that are cut at different steps, a long prompt in chunks
+    (cut between them too) and one that joins later."""
+    eng = LLMEngine(_cfg(max_num_batched_tokens=24))
+    prompts = [list(range(10, 100)), list(range(30, 50)), [9, 8, 7, 6]]
+    ids = [eng.add_request(p, SP) for p in prompts[:2]]
+    for _ in range(9):
+        eng.step()
+    ids.append(eng.add_request(prompts[2], SP))
+    most = 0
+    while eng.has_unfinished():
+        eng.step()
+        most = max([most] + [len(s.block_table) for s in eng.scheduler.running])
+    # 32 + 8 keys and the one that comes
+    assert most <= -(-42 // 16)
+    assert eng.seqs[ids[0]].output_token_ids == _replayed(
+        eng, prompts[0], 60, monkeypatch, chunk=24)
+    for i in (1, 2):
+        assert eng.seqs[ids[i]].output_token_ids == _replayed(
+            eng, prompts[i], 60, monkeypatch)
+    assert eng.pool.num_free == eng.pool.num_blocks
+
+
+def test_preempted_sequences_begin_anew():
+    """A pool that runs dry: victims lose their cuts with their caches, and
+    every sequence ends with all of its tokens and the pages given back."""
+    eng = LLMEngine(_cfg(num_gpu_blocks=7, max_num_seqs=4, max_model_len=96))
+    ids = [eng.add_request(list(range(a, a + 14)), SP) for a in (10, 30, 50)]
+    for _ in range(500):
+        if not eng.has_unfinished():
+            break
+        eng.step()
+    assert any(eng.seqs[i].epoch > 0 for i in ids)
+    assert all(len(eng.seqs[i].output_token_ids) == 60 for i in ids)
+    assert eng.pool.num_free == eng.pool.num_blocks
+
+
+@pytest.mark.parametrize("kw", [
+    dict(kv_budget=0), dict(kv_budget_recent=33), dict(kv_budget_slack=-1),
+    dict(kv_budget_recent=-1), dict(enable_mixed_batch=True),
+    dict(model=get_model_config("tiny-deepseek-test")),
+    dict(model=dataclasses.replace(get_model_config("tiny-llama-test"),
+                                   sliding_window=32,
+                                   sliding_window_pattern="all"))])
+def test_refused(kw):
+    with pytest.raises(ValueError):
+        LLMEngine(_cfg(**kw))
+
+
+def test_what_a_budget_turns_off():
+    eng = LLMEngine(_cfg(enable_prefix_caching=True, kv_offload=True))
+    assert not hasattr(eng.pool, "match_prefix") and eng.kv_offload is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eager", [True, False])
+@pytest.mark.parametrize("dtype", ["auto", "fp8"])
+def test_serving_on_the_gpu(eager, dtype):
+    """With graphs and without: the same tokens, and those of an engine
+    without a budget while nothing is cut."""
+    kw = dict(device="cuda", enforce_eager=eager, kv_cache_dtype=dtype,
+              graph_batch_sizes=(1, 2, 4), max_num_seqs=4)
+    prompts = [list(range(10, 100)), [3, 5, 7, 11]]
+    eng = LLMEngine(_cfg(**kw)).capture_graphs()
+    got = eng.generate(prompts, SP)
+    assert all(s.evicted > 0 for s in got)
+    assert eng.pool.num_free == eng.pool.num_blocks
+    again = LLMEngine(_cfg(**dict(kw, enforce_eager=True))).generate(prompts, SP)
+    for a, b in zip(got, again):
+        assert a.output_token_ids == b.output_token_ids
+    short = SamplingParams(max_tokens=20, ignore_eos=True)
+    wide = LLMEngine(_cfg(**dict(kw, kv_budget=200))).capture_graphs()
+    for s in wide.generate(prompts, short):
+        assert s.evicted == 0 and len(s.output_token_ids) == 20
