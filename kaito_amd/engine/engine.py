@@ -124,6 +124,8 @@ class LLMEngine:
         if st.pp_size > 1 or cfg.enable_mixed_batch or cfg.block_size != 16:
             raise ValueError("kv_budget needs pages of 16 keys, one pipeline "
                              "stage and no mixed steps")
+        if str(cfg.device) != "cpu" and m.dtype != torch.bfloat16:
+            raise ValueError(f"kv_budget: no kernels for {m.dtype}")
         if str(cfg.device) != "cpu" and not (
                 m.head_dim == 128 and group <= 8
                 or m.head_dim == 64 and group in (1, 2, 4, 8)

@@ -176,8 +176,10 @@ void flash_prefill_kernel(const Args a) {
   if ((QP > TILE && (q0 & (QP - 1))) || q0 >= q_len) return;
   const int h0 = hg << a.gs;
   const int kvh = h0 / (a.QH / a.KH);
+  // STATS: never more keys than the table holds, as in the pass behind it
   const int q_abs0 = a.starts ? a.starts[seq]
-      : (a.kv_lens ? a.kv_lens[seq] - q_len : 0);
+      : (a.kv_lens ? (STATS ? min(a.kv_lens[seq], a.max_blocks * a.BS)
+                            : a.kv_lens[seq]) - q_len : 0);
   const int kv_len = q_abs0 + q_len;
   const int* bt = SRC == ROWS_BF16 ? nullptr
       : a.block_tables + (int64_t)seq * a.max_blocks;

@@ -256,6 +256,47 @@ def test_heavy_keys(dev, budget, recent, kind):
     assert n.tolist() == [min(L, budget) for L in lens]
 
 
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+def test_heavy_keys_of_many_heads(dev):
+    """More kv heads than a short cache's choice sums by itself."""
+    lens = [700, 33]
+    _, _, w, tables = _pages(lens, 20, 64)
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    kept, _ = ops.heavy_keys(w.to(dev), tables.to(dev), n, 200, 10)
+    assert torch.equal(kept.cpu(), _heavy(w, tables, lens, 200, 10))
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+def test_nothing_to_do(dev):
+    """No sequences; tables without pages; no new rows at all."""
+    k, v, w, tables = (t.to(dev) for t in _pages([40], 2, 64))
+    before = [t.clone() for t in (k, v, w)]
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=dev)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    zero = torch.zeros(1, dtype=torch.int32, device=dev)
+    nothing = zero.new_zeros(0, 3)
+    assert ops.paged_attention_weights(q, k, v, w, nothing, none,
+                                       1.0).shape == q.shape
+    assert ops.context_attention_weights(q, k, v, w, zero, none, nothing,
+                                         1.0).shape == q.shape
+    cu = torch.zeros(2, dtype=torch.int32, device=dev)
+    assert ops.context_attention_weights(q, k, v, w, cu, zero + 40, tables,
+                                         1.0).shape == q.shape
+    kept, n = ops.heavy_keys(w, nothing, none, 8, 2)
+    assert kept.shape == (0, 8) and n.shape == (0,)
+    ops.compact_pages(k, v, w, nothing, kept, n)
+    # a row whose table has no pages
+    one = torch.ones(1, 4, 64, dtype=torch.bfloat16, device=dev)
+    empty = zero.new_zeros(1, 0)
+    assert (ops.paged_attention_weights(one, k, v, w, empty, zero, 1.0)
+            == 0).all()
+    kept, n = ops.heavy_keys(w, empty, zero, 8, 2)
+    assert (kept == -1).all() and n.tolist() == [0]
+    ops.compact_pages(k, v, w, empty, kept, n)
+    for a, b in zip((k, v, w), before):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens,budget,recent", [([40000, 39999], 20000, 100),
                                                 ([70001], 1000, 999),
