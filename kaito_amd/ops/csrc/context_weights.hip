@@ -22,7 +22,9 @@
 // flash_prefill.h's twice as many. One product after another and then all weights
 // 381 us; the loop without masks and addresses 315; products and weights in turns
 // 298; tiles of 64 rows and fragments four products ahead of their use 268. Eight
-// waves that share a tile: 278.
+// waves that share a tile: 278. Products of 16 x 16 x 32, of which two take 18 ns by
+// themselves and as many multiply-adds and exponentials in between 25: 287 (276 with
+// those gathered by fours), without copies and barriers 258, without LDS reads 222.
 #include "flash_prefill.h"
 #include "keys_common.h"
 #include <torch/library.h>

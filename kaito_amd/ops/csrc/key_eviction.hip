@@ -2,16 +2,26 @@
 //
 // heavy_keys: a sequence of more than `budget` keys keeps its newest `recent` and
 //   the budget - recent others with the largest weights, summed over the kv heads.
-//   key_total_kernel: one thread per key sums its heads in f64 and leaves the f32
-//   total as an integer of the same order. choose_keys_kernel: one workgroup per
-//   sequence finds the smallest total that stays, eight bits at a time (a histogram
-//   in LDS per digit), and writes the places of those above it and of as many equal
-//   ones as there is room for, lowest places first, by ballots and a running count.
-//   No step depends on timing.
+//   Totals, in f64 and rounded to f32, become integers of the same order
+//   (key_total_kernel; for short tables the choosing launch itself). choose_keys_kernel:
+//   one workgroup per sequence keeps them in registers, 2048 bins over the range of
+//   totals at a time narrow down the smallest one that stays until 64 are left, which
+//   one wave ranks; then the places of those above it and of as many equal ones as
+//   there is room for, lowest places first, from ballots and a running sum. No step
+//   depends on timing.
 // compact_pages: key kept[i] goes to place i, in place. `kept` ascends, so that
 //   kept[i] >= i, and the sources of later places are never among earlier ones: a
 //   workgroup per sequence, kv head and array takes its places tile by tile, a
 //   barrier between a tile's loads and its stores, and nothing else has to wait.
+//
+// What bounds them: the choice is a chain of short steps in one workgroup (load and
+// sum 3.7 us, ends 1.4, a level of bins 1.3, the last few 0.3, places 1.6, the launch
+// of 16 waves the rest): 12.4 us for 64 caches of 4352 keys and 8 kv heads, 22 with
+// its totals for 4 of 32768; by eight bits of the total at a time 15 and 71, as the
+// totals of a cache share their leading bits and queued for a few bins. The closing
+// is bound by memory where there are caches enough: 64 of 4352 keys, 8 kv heads of
+// 128, 481 us, 4.5 TB/s read and written (one load of a thread under way 609); 4 of
+// 700 6.2 us (20), by columns that make 512 workgroups.
 #include "common.h"
 #include "keys_common.h"
 #include <torch/library.h>
@@ -106,27 +116,28 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
   for (int i = tid; i < recent; i += CHOOSERS) out[heavy + i] = old + i;
   if (heavy == 0) return;
 
+  // rows of CHOOSERS keys, by fours: those behind the last are not gone through
+#define EACH_ROW(BASE_)                                                       \
+  _Pragma("unroll")                                                           \
+  for (int j0 = 0; j0 < PER && (BASE_) + j0 * CHOOSERS < old; j0 += 4)        \
+    _Pragma("unroll") for (int j = j0; j < j0 + (PER < 4 ? PER : 4); j++)
   unsigned x[PER];                  // keys base + j * CHOOSERS + tid
   auto load = [&](const int base) {
     if constexpr (SUMS) {
       const int* bt = block_tables + (int64_t)seq * width;
       const float* at[PER];
       double sum[PER];
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
+      EACH_ROW(base) {
         const int i = min(base + j * CHOOSERS + tid, old - 1);
         at[j] = key_weights + (int64_t)bt[i / PAGE] * KH * PAGE + i % PAGE;
         sum[j] = 0.;
       }
 #pragma unroll 4
       for (int h = 0; h < KH; h++)
-#pragma unroll
-        for (int j = 0; j < PER; j++) sum[j] += (double)at[j][h * PAGE];
-#pragma unroll
-      for (int j = 0; j < PER; j++) x[j] = ordered((float)sum[j]);
+        EACH_ROW(base) sum[j] += (double)at[j][h * PAGE];
+      EACH_ROW(base) x[j] = ordered((float)sum[j]);
     } else {
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
+      EACH_ROW(base) {
         const int i = base + j * CHOOSERS + tid;
         x[j] = i < old ? w[i] : 0u;
       }
@@ -143,8 +154,7 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
   // ---- smallest and largest total
   unsigned lo = ~0u, hi = 0u;
   parts([&](const int base) {
-#pragma unroll
-    for (int j = 0; j < PER; j++)
+    EACH_ROW(base)
       if (base + j * CHOOSERS + tid < old) {
         lo = min(lo, x[j]);
         hi = max(hi, x[j]);
@@ -173,8 +183,7 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
       const int first = (x[0] - lo) >> shift;
       const bool alike = __popcll(__ballot(
           first == __builtin_amdgcn_readfirstlane(first))) > 16;
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
+      EACH_ROW(base) {
         const unsigned d = x[j] - lo;
         if (d > hi - lo || base + j * CHOOSERS + tid >= old) continue;
         const int bin = d >> shift;
@@ -213,8 +222,7 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
     if (tid == 0) listed = 0;
     __syncthreads();
     parts([&](const int base) {
-#pragma unroll
-      for (int j = 0; j < PER; j++)
+      EACH_ROW(base)
         if (base + j * CHOOSERS + tid < old && x[j] >= lo && x[j] <= hi)
           few[atomicAdd(&listed, 1)] = x[j];
     });
@@ -242,8 +250,7 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
   int at = 0, ties = 0;             // kept and equal ones before this part
   __syncthreads();
   parts([&](const int base) {
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
+    EACH_ROW(base) {
       const bool in = base + j * CHOOSERS + tid < old;
       const int t = __popcll(__ballot(in && x[j] - lo <= hi - lo));
       const int m = __popcll(__ballot(in && x[j] > hi));
@@ -256,18 +263,17 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
     if (wave < 2) {                 // running sums, in the order of the keys
       int* c = counts[wave];
       int before = 0;
-#pragma unroll
-      for (int k = 0; k < PER * WAVES; k += 64) {
-        const int n = k + lane < PER * WAVES ? c[k + lane] : 0;
+      const int rows = min(PER, (old - base + 4 * CHOOSERS - 1) / (4 * CHOOSERS) * 4);
+      for (int k = 0; k < rows * WAVES; k += 64) {
+        const int n = k + lane < rows * WAVES ? c[k + lane] : 0;
         const int sum = lanes_up_to(n, Plus{});
-        if (k + lane < PER * WAVES) c[k + lane] = before + sum - n;
+        if (k + lane < rows * WAVES) c[k + lane] = before + sum - n;
         before += __builtin_amdgcn_readlane(sum, 63);
       }
       if (lane == 0) found[wave] = before;
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
+    EACH_ROW(base) {
       const int i = base + j * CHOOSERS + tid;
       const bool tie = i < old && x[j] - lo <= hi - lo;
       const bool more = i < old && x[j] > hi;
@@ -282,6 +288,7 @@ void choose_keys_kernel(int* __restrict__ kept, int* __restrict__ kept_lens,
     __syncthreads();
   });
 }
+#undef EACH_ROW
 
 constexpr int MOVERS = 256;
 constexpr int DEEP = 8;             // loads of a thread under way at once
