@@ -16,9 +16,10 @@
 //
 // What bounds them: the choice is a chain of short steps in one workgroup (load and
 // sum 3.7 us, ends 1.4, a level of bins 1.3, the last few 0.3, places 1.6, the launch
-// of 16 waves the rest): 12.4 us for 64 caches of 4352 keys and 8 kv heads, 22 with
-// its totals for 4 of 32768; by eight bits of the total at a time 15 and 71, as the
-// totals of a cache share their leading bits and queued for a few bins. The closing
+// of 16 waves the rest): 10.5 us for 64 caches of 4352 keys and 8 kv heads, 23 with
+// its totals for 4 of 32768, 15 for 16 of 6000 to 9000; by eight bits of the total at a
+// time 15 and 71, as the totals of a cache share their leading bits and queued for a
+// few bins; with all rows of registers gone through 12.7, 22 and 21. The closing
 // is bound by memory where there are caches enough: 64 of 4352 keys, 8 kv heads of
 // 128, 481 us, 4.5 TB/s read and written (one load of a thread under way 609); 4 of
 // 700 6.2 us (20), by columns that make 512 workgroups.
