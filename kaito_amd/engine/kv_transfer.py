@@ -50,8 +50,10 @@ def extract_kv(kv_caches, block_table: List[int], n_tokens: int,
 
 def inject_kv(kv_caches, block_table: List[int],
               layers: List[Tuple[torch.Tensor, torch.Tensor]],
-              block_size: int) -> None:
-    """Scatter transferred KV into the receiving pool's blocks."""
+              block_size: int, key_weights=None) -> None:
+    """Scatter transferred KV into the receiving pool's blocks. An engine with
+    a kv_budget gives its runner's key_weights: keys that come from elsewhere
+    have received nothing here."""
     n = layers[0][0].shape[1]
     nb = (n + block_size - 1) // block_size
     dev = kv_caches[0][0].device
@@ -65,6 +67,8 @@ def inject_kv(kv_caches, block_table: List[int],
         vp[:, :n] = v.to(dev)
         kc[blocks] = kp.reshape(kvh, nb, block_size, d).permute(1, 0, 2, 3)
         vc[blocks] = vp.reshape(kvh, nb, block_size, d).permute(1, 0, 2, 3)
+    for w in key_weights or ():
+        w[blocks] = 0
 
 
 # --------------------------------------------------------------- connectors

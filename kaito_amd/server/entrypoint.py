@@ -42,7 +42,8 @@ def build_parser() -> argparse.ArgumentParser:
                    help="keys that a sequence's cache keeps per layer: "
                         "beyond them (and a slack of 128) those that have "
                         "received the least attention are cut, the newest "
-                        "256 never (no prefix caching, no swap space)")
+                        "256 (half of a smaller budget) never; no prefix "
+                        "caching and no swap space then")
     p.add_argument("--enable-kv-events", action="store_true",
                    help="publish BlockStored/BlockRemoved on :5557 "
                         "(EPP KVCache-aware routing)")
@@ -142,6 +143,7 @@ def main(argv=None):
         kv_cache_dtype=("fp8" if args.kv_cache_dtype in
                         ("fp8", "fp8_e4m3") else "auto"),
         kv_budget=args.kv_budget,
+        kv_budget_recent=min(256, (args.kv_budget or 512) // 2),
     )
     if args.kv_cache_dtype not in ("auto", "bf16", "bfloat16", "fp8",
                                    "fp8_e4m3"):

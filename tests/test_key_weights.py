@@ -193,6 +193,33 @@ def test_token_launch_rules(D, KH, lens, width, fp8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", [(7, 1, 128), (16, 2, 128), (4, 4, 64),
+                                    (3, 1, 128)])
+def test_tokens_of_other_groups_in_splits(layout):
+    _run("cuda", layout, [1] * 4, [2499, 8, 1300, 0], sinks=True, width=260,
+         token=True, seed=9)
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+def test_scales_that_are_not_positive(dev, scale):
+    """Every visible key alike, and the least alike first."""
+    new, past = [40, 3], [300, 0]
+    lens = [a + b for a, b in zip(new, past)]
+    k, v, w, tables = _pages(lens, 2, 64)
+    q = torch.randn(43, 4, 64).bfloat16()
+    want, near, want_w, off = _oracle(q, k, v, w, new, lens, tables, scale, None)
+    cu = torch.tensor([0, 40, 43], dtype=torch.int32)
+    got = w.to(dev)
+    out = ops.context_attention_weights(
+        q.to(dev), k.to(dev), v.to(dev), got, cu.to(dev),
+        torch.tensor(lens, dtype=torch.int32).to(dev), tables.to(dev), scale)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20).all()
+    assert ((got.cpu().double() - want_w).abs() <= off)[off > 0].all()
+
+
+@pytest.mark.gpu
 def test_scores_without_a_weight():
     """Keys whose scores are minus infinity receive nothing, and a row that has
     no other key changes no entry."""

@@ -163,6 +163,18 @@ def test_refused(kw):
         LLMEngine(_cfg(**kw))
 
 
+def test_transferred_keys_have_received_nothing():
+    from kaito_amd.engine.kv_transfer import extract_kv, inject_kv
+    a, b = LLMEngine(_cfg()), LLMEngine(_cfg())
+    for w in b.runner.key_weights:
+        w.fill_(7.)
+    pages = b.pool.allocate(2)
+    layers = extract_kv(a.runner.kv_caches, a.pool.allocate(2), 20, 16)
+    inject_kv(b.runner.kv_caches, pages, layers, 16, b.runner.key_weights)
+    for w in b.runner.key_weights:
+        assert (w[pages] == 0).all() and (w.sum() > 0)
+
+
 def test_what_a_budget_turns_off():
     eng = LLMEngine(_cfg(enable_prefix_caching=True, kv_offload=True))
     assert not hasattr(eng.pool, "match_prefix") and eng.kv_offload is None
