@@ -167,6 +167,15 @@ def test_few_rows_over_many_keys(layout, sinks):
     _run("cuda", layout, [3], [13], sinks=sinks, width=600)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 63, 64, 65])
+def test_many_chunks(seqs):
+    """Sequences by the lengths of their chunks, equal ones among them; enough
+    keys for workgroups of 256."""
+    _run("cuda", (4, 2, 64), [(7 * i) % 13 for i in range(seqs)],
+         [(31 * i) % 97 for i in range(seqs)], width=900 // seqs * 8, seed=seqs)
+
+
 @pytest.mark.parametrize("dev", CPU_OR_GPU)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("fp8", [False, True])
