@@ -505,9 +505,10 @@ class ModelRunner:
                     b["block_tables"][i, :n].copy_(torch.tensor(
                         s.block_table, dtype=torch.int32), non_blocking=True)
                     s._bt_dirty = False
-            # slot = bt[i, key // BS] * BS + key % BS  (device-side gather) of
-            # the row's own key, its cache's last
-            pos = b["seq_lens"][:bs].long() - 1
+            # slot = bt[i, pos // BS] * BS + pos % BS  (device-side gather);
+            # in cut caches the row's own key is the last that they hold
+            pos = b["positions"][:bs] if self.key_weights is None \
+                else b["seq_lens"][:bs].long() - 1
             blk = torch.gather(b["block_tables"][:bs].long(), 1,
                                (pos // self.cfg.block_size).unsqueeze(1)).squeeze(1)
             b["slot_mapping"][:bs].copy_(
@@ -520,7 +521,9 @@ class ModelRunner:
             narrow[1:3] = -1
             dst, src = [], []
             lens = [s.sched_tokens for s in seqs]
-            keys = np.array([n - s.evicted for n, s in zip(lens, seqs)])
+            keys = np.array(lens)
+            if self.key_weights is not None:
+                keys -= [s.evicted for s in seqs]
             bsz = self.cfg.block_size
             flat = np.zeros((bs, self._max_blocks), dtype=np.int32)
             for i, s in enumerate(seqs):
