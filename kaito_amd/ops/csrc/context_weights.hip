@@ -493,8 +493,12 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
   TORCH_CHECK(G <= ROWS, "unsupported GQA group ", G);
   TORCH_CHECK(T < (1ll << 31), "q: too many rows");
   TORCH_CHECK(q.stride(0) < (1 << 25), "q: rows 2^25 apart at most");
-  if (ntiles == 0 || T == 0 || block_tables.size(1) == 0) return;
+  if (ntiles == 0 || T == 0) return;
   const keys::Guard guard(q.device());
+  if (block_tables.size(1) == 0) {  // no row has a key
+    out.zero_();
+    return;
+  }
   const at::Tensor stats = at::empty({T, a.QH, 2}, q.options().dtype(at::kFloat));
   a.BS = keys::PAGE;
   a.max_blocks = block_tables.size(1);

@@ -156,6 +156,7 @@ void flash_prefill_kernel(const Args a) {
   constexpr int CK = D / 8, CV = DV / 8;          // 16-byte chunks of a row
   constexpr int NT = NW * 64, ROWS = NW * 32;     // threads, query rows
   constexpr int LK = KVT * CK / NT, LV = KVT * CV / NT;
+  constexpr bool PAGED = SRC != ROWS_BF16;
   // with nothing but a positive factor between product and exponent, it
   // rides in the exponent's multiply-add
   const bool fold = !EXT && !SIG && !DB && a.scale > 0.f;
@@ -244,11 +245,22 @@ void flash_prefill_kernel(const Args a) {
         ((kv_end + KVT - 1) / KVT + a.splits - 1) / a.splits * KVT;
     kv_first = split * share;
     kv_end = min(kv_end, kv_first + share);
-    if (kv_first >= kv_end) {
+    if (kv_first >= kv_end && a.splits > 1) {
       if (h == 0 && qrow < q_len)
         a.stats[((int64_t)split * a.rows + tok0 + qrow) * a.QH + head] = {m, l};
       return;
     }
+  }
+  // Rows that see no key come out as zeros. Without a key there is no page to look
+  // up, so that they end here.
+  if (PAGED && kv_end <= 0) {
+    if (qrow >= q_len) return;
+    if (STATS && h == 0)
+      a.stats[((int64_t)tok0 + qrow) * a.QH + head] = {m, 1.f};
+    short* orow = a.out + ((int64_t)(tok0 + qrow) * a.QH + head) * DV;
+    for (int d = h * 8; d < DV; d += 16)
+      *reinterpret_cast<short8_t*>(orow + d) = short8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    return;
   }
   auto next_tile = [&](const int kv0) {
     return EXT && kv0 + KVT == first_end ? kv_begin : kv0 + KVT;
@@ -266,7 +278,6 @@ void flash_prefill_kernel(const Args a) {
   // size 256, 118 -> 107 us. The same for rows of the step gave 3 % at 8192 and
   // took 2 % at 4 x 2048.
   static_assert(SRC == ROWS_BF16 || (64 % CK == 0 && 64 % CV == 0));
-  constexpr bool PAGED = SRC != ROWS_BF16;
   // The distance bias at 128 x 128 has no registers left for it: 13 spilled, 4 x
   // 2048, 16/4 heads, window 1024: 128.7 -> 139.8 us.
   constexpr bool SCALAR_PAGES = PAGED && !(DB && D == 128 && DV == 128);

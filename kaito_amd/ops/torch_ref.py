@@ -211,7 +211,7 @@ def _add_key_weights(key_weights, block_table, L: int, new: int, p):
     j = torch.arange(L, device=p.device)
     pages = block_table[j // BS].long()
     old = key_weights[pages, :, j % BS]                            # [L, KH]
-    old[L - new:] = 0
+    old[max(L - new, 0):] = 0
     w = p.unflatten(0, (KH, -1)).sum((1, 2)).T
     key_weights[pages, :, j % BS] = old + w.to(key_weights.dtype)
 
@@ -246,6 +246,7 @@ def context_attention_weights(q, k_cache, v_cache, key_weights, cu_seqlens_q,
             s = torch.cat([s, sinks.float()[:, None, None].expand(-1, n, 1)],
                           dim=-1)
         p = torch.softmax(s, dim=-1)[..., :L]
+        p[:, :max(n - L, 0)] = 0        # rows ahead of the first key see none
         out[cs[b]:cs[b + 1]] = (p @ v).transpose(0, 1).to(q.dtype)
         _add_key_weights(key_weights, block_tables[b], L, n, p)
     return out

@@ -642,3 +642,42 @@ def test_strided_arguments():
     ops.compact_pages(*other, tables, kept, left)
     for s, t in zip((k, v, a), other):
         assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("D,fp8", [(64, True), (128, False), (256, False)])
+@pytest.mark.parametrize("width,said", [
+    (None, 40),             # keys in one share
+    (64, 40),               # in several
+    (800, 40),              # and workgroups of 256 keys
+    (2, 4000),              # a table that ends before the keys do
+    (0, 40)])               # and one without pages
+def test_rows_that_see_no_key(dev, D, fp8, width, said):
+    """More rows than keys, and rows of a sequence without any: zeros where a row
+    sees nothing, the rest as ever."""
+    QH, KH, new = 2, 1, [200, 9, 1]
+    held = said if width is None or width > 2 else width * PAGE
+    lens = [held, 0, min(held, 1)]
+    k, v, w, tables = _pages(lens, KH, D, fp8, width)
+    if width == 0:
+        tables = tables[:, :0]
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(sum(new), QH, D, generator=g).bfloat16()
+    scale = D ** -0.5
+    live = torch.cat([torch.arange(n) >= n - m for n, m in zip(new, lens)])
+    want, near, want_w, off = _oracle(q[live], k, v, w, lens, lens, tables, scale,
+                                      None)
+    q = q.to(dev)
+    got, cu, lens = (t.to(dev) for t in (
+        w, torch.tensor([0] + new).cumsum(0).int(),
+        torch.tensor([said] + lens[1:], dtype=torch.int32)))
+    k, v, tables = (t.to(dev) for t in (k, v, tables))
+    torch.full(q.shape, math.nan, dtype=q.dtype, device=dev)    # taken next
+    out = ops.context_attention_weights(q, k, v, got, cu, lens, tables, scale)
+    out, got = out.cpu().double(), got.cpu().double()
+    assert (out[~live] == 0).all()
+    err = (out[live] - want).abs()
+    assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20).all()
+    assert ((got - want_w).abs() <= off)[off > 0].all()
+    assert torch.equal(got[off == 0].float().view(torch.int32),
+                       w[off == 0].view(torch.int32))
