@@ -245,9 +245,9 @@ void flash_prefill_kernel(const Args a) {
         ((kv_end + KVT - 1) / KVT + a.splits - 1) / a.splits * KVT;
     kv_first = split * share;
     kv_end = min(kv_end, kv_first + share);
-    if (kv_first >= kv_end && a.splits > 1) {
+    if (kv_first >= kv_end && a.splits > 1) {   // no output: a sink has no part in it
       if (h == 0 && qrow < q_len)
-        a.stats[((int64_t)split * a.rows + tok0 + qrow) * a.QH + head] = {m, l};
+        a.stats[((int64_t)split * a.rows + tok0 + qrow) * a.QH + head] = {m, 0.f};
       return;
     }
   }

@@ -652,7 +652,8 @@ def test_strided_arguments():
     (800, 40),              # and workgroups of 256 keys
     (2, 4000),              # a table that ends before the keys do
     (0, 40)])               # and one without pages
-def test_rows_that_see_no_key(dev, D, fp8, width, said):
+@pytest.mark.parametrize("sinks", [False, True])
+def test_rows_that_see_no_key(dev, D, fp8, width, said, sinks):
     """More rows than keys, and rows of a sequence without any: zeros where a row
     sees nothing, the rest as ever."""
     QH, KH, new = 2, 1, [200, 9, 1]
@@ -664,16 +665,23 @@ def test_rows_that_see_no_key(dev, D, fp8, width, said):
     g = torch.Generator().manual_seed(4)
     q = torch.randn(sum(new), QH, D, generator=g).bfloat16()
     scale = D ** -0.5
+    sink = torch.randn(QH, generator=g) if sinks else None
     live = torch.cat([torch.arange(n) >= n - m for n, m in zip(new, lens)])
     want, near, want_w, off = _oracle(q[live], k, v, w, lens, lens, tables, scale,
-                                      None)
+                                      sink)
     q = q.to(dev)
     got, cu, lens = (t.to(dev) for t in (
         w, torch.tensor([0] + new).cumsum(0).int(),
         torch.tensor([said] + lens[1:], dtype=torch.int32)))
     k, v, tables = (t.to(dev) for t in (k, v, tables))
-    torch.full(q.shape, math.nan, dtype=q.dtype, device=dev)    # taken next
-    out = ops.context_attention_weights(q, k, v, got, cu, lens, tables, scale)
+    if sinks:
+        sink = sink.to(dev)
+    # what is taken next: the output and, for several shares, theirs
+    old = [torch.full(q.shape, math.nan, dtype=q.dtype, device=dev),
+           torch.full((2 << 20,), math.nan, device=dev)]
+    del old
+    out = ops.context_attention_weights(q, k, v, got, cu, lens, tables, scale,
+                                        sink)
     out, got = out.cpu().double(), got.cpu().double()
     assert (out[~live] == 0).all()
     err = (out[live] - want).abs()
