@@ -431,12 +431,13 @@ template <int D, int WPR>
 __global__ __launch_bounds__(256)
 void join_kernel(short* __restrict__ out, float2* __restrict__ stats,
                  const float2* __restrict__ parts, const float* __restrict__ part,
-                 const int splits, const int64_t rows) {
+                 const int* __restrict__ ends, const int QH, const int splits,
+                 const int64_t rows) {
   constexpr int EACH = D / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   __shared__ float sums[WPR == 1 ? 1 : WPR][D];
-  if (row >= rows) return;          // with WPR > 1 none
+  if (row >= (int64_t)*ends * QH) return;       // behind the last sequence: not ours
   const float2 mine = parts[min(lane, splits - 1) * rows + row];
   const float m = wave_reduce_max(mine.x);
   // a share whose sum is 0 has left no output; one that is no number does count
@@ -560,7 +561,7 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
     auto join = [&](auto kernel, const int64_t groups) {
       hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, a.out,
                          (float2*)stats.data_ptr<float>(), a.stats, a.part,
-                         a.splits, rows);
+                         a.cu + B, a.QH, a.splits, rows);
     };
     if (a.splits > 8) join(join_kernel<D_, 4>, rows);
     else if (a.splits > 1) join(join_kernel<D_, 1>, (rows + 3) / 4);

@@ -689,3 +689,20 @@ def test_rows_that_see_no_key(dev, D, fp8, width, said, sinks):
     assert ((got - want_w).abs() <= off)[off > 0].all()
     assert torch.equal(got[off == 0].float().view(torch.int32),
                        w[off == 0].view(torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [None, 64, 300])
+def test_rows_behind_the_last_sequence(width):
+    """Rows of a padded step that belong to no sequence stay as they were, in one
+    share of the keys and in several."""
+    k, v, w, tables = (t.cuda() for t in _pages([40], 1, 128, width=width))
+    q = torch.randn(20, 2, 128).bfloat16().cuda()
+    cu = torch.tensor([0, 7], dtype=torch.int32).cuda()
+    lens = torch.tensor([40], dtype=torch.int32).cuda()
+    own = ops.context_attention_weights(q[:7], k, v, w.clone(), cu, lens, tables, 0.1)
+    seq, base = ops.build_query_tiles([7], "cuda")
+    out = torch.full_like(q, 7.)
+    ops._K.context_attention_weights(out, q, k, v, w, seq, base, cu, lens, tables,
+                                     0.1, torch.empty(0, device="cuda"))
+    assert torch.equal(out[:7], own) and (out[7:] == 7).all()
