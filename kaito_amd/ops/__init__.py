@@ -981,7 +981,9 @@ def context_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
     chunk's own rows (the last of kv_lens) begin anew, so that a page's entries
     need no clearing when it changes hands. A sequence without rows changes
     nothing; a row that sees no key (kv_lens below the number of rows, a table
-    that ends before them) comes out as zeros. Pages are a sequence's own here: what becomes of the weights of one
+    that ends before them) comes out as zeros. A score that is no number, or
+    infinite, makes its row's output NaN and the entries of all keys that the
+    row sees. Pages are a sequence's own here: what becomes of the weights of one
     that two tables of a call share is not defined. q bf16 of any strides, head
     sizes 64, 128 and 256, bf16 or e4m3 pages of 16 keys."""
     if q.is_cuda:

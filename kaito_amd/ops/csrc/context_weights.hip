@@ -440,10 +440,12 @@ void join_kernel(short* __restrict__ out, float2* __restrict__ stats,
   if (row >= (int64_t)*ends * QH) return;       // behind the last sequence: not ours
   const float2 mine = parts[min(lane, splits - 1) * rows + row];
   const float m = wave_reduce_max(mine.x);
-  // a share whose sum is 0 has left no output; one that is no number does count
-  const float e = lane < splits && mine.y != 0.f
-      ? __builtin_amdgcn_exp2f(mine.x - m) : 0.f;
-  const float inv = 1.f / fmaxf(wave_reduce_sum(e == 0.f ? 0.f : e * mine.y), 1e-30f);
+  // a share whose sum is 0 has left no output; one that is no number counts, however
+  // small its maximum
+  const float e = lane >= splits || mine.y == 0.f ? 0.f
+      : mine.y == mine.y ? __builtin_amdgcn_exp2f(mine.x - m) : mine.y;
+  const float sum = wave_reduce_sum(e == 0.f ? 0.f : e * mine.y);
+  const float inv = 1.f / fmaxf(sum, 1e-30f);
   float o[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; i++) o[i] = 0.f;
@@ -468,7 +470,7 @@ void join_kernel(short* __restrict__ out, float2* __restrict__ stats,
 #pragma unroll
   for (int i = 0; i < EACH; i++)
     out[row * D + lane * EACH + i] = f32_to_bf16(o[i] * inv);
-  if (lane == 0) stats[row] = {m, inv};
+  if (lane == 0) stats[row] = {sum == sum ? m : sum, inv};
 }
 
 }  // namespace

@@ -619,7 +619,10 @@ void flash_prefill_kernel(const Args a) {
   float inv = 1.0f / fmaxf(l, 1e-30f);
   if constexpr (STATS) {
     const int64_t at = ((int64_t)split * a.rows + tok0 + qrow) * a.QH + head;
-    if (h == 0) a.stats[at] = {m, a.splits > 1 ? l : inv};
+    // a sum that is no number makes every weight of the row none: m does, as 1 / l
+    // would reach keys that the row does not see
+    if (h == 0)
+      a.stats[at] = a.splits > 1 ? float2{m, l} : float2{l == l ? m : l, inv};
     if (a.splits > 1) {
       float* orow = a.part + at * DV + 4 * h;
 #pragma unroll

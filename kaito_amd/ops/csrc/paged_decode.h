@@ -224,6 +224,12 @@ KAITO_DEV Spans spans_of(const int seq_len, const int window, const int nsplit,
   return p;
 }
 
+// KEEP: what a weight is made of its score with, maximum and 1 / sum: none where the
+// sum is none
+KAITO_DEV float2 keep_of(const float m, const float sum) {
+  return {sum == sum ? m : sum, 1.f / fmaxf(sum, 1e-20f)};
+}
+
 // KEEP: what four keys, of one page, receive from the heads of a group, given their
 // maxima and 1 / sums; the row's own key begins anew. Scores behind `len` are there,
 // weights are not touched. One thread per four keys and kv head.
@@ -244,7 +250,7 @@ KAITO_DEV void add_key_weights(const DecodeArgs& a, const int64_t row,
     const float2 st = stats[g];
 #pragma unroll
     for (int i = 0; i < 4; i++)     // what the attention gives no weight has none here
-      if (x[i] > -1e29f)
+      if (!(x[i] <= -1e29f))        // what is no number is one in the entry
         sum[i] += __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
   };
   int g = 0;
@@ -496,8 +502,9 @@ void paged_decode_kernel(const DecodeArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           // a masked key weighs nothing even where a lane saw no other yet; so
-          // does one whose score is -infinity
-          const bool live = BIASED ? s[i][r] != NONE : s[i][r] > -1e29f;
+          // does one whose score is -infinity and, but with KEEP, no number
+          const bool live = BIASED ? s[i][r] != NONE
+              : KEEP ? !(s[i][r] <= -1e29f) : s[i][r] > -1e29f;
           float w = live ? fold_weight<BIASED>(s[i][r], m) : 0.f;
           l += w;
 #pragma unroll
@@ -616,7 +623,7 @@ void paged_decode_kernel(const DecodeArgs a) {
     } else {
       if (a.sinks) den += fold_weight<BIASED>(sink, gm);
       if constexpr (KEEP)
-        if (d == 0) s_keep[g] = {gm, 1.f / fmaxf(den, 1e-20f)};
+        if (d == 0) s_keep[g] = keep_of(gm, den);
       store_head<BIASED>(a, seq, QH, head, D, d, num, den);
     }
   }
@@ -697,7 +704,7 @@ void paged_fold_weights_kernel(const DecodeArgs a, const int splits) {
     s_e[g][lane] = e;
     if (lane == 0) {
       s_den[g] = den;
-      s_keep[g] = {gm, 1.f / fmaxf(den, 1e-20f)};
+      s_keep[g] = keep_of(gm, den);
     }
   }
   __syncthreads();

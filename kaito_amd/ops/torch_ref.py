@@ -245,8 +245,8 @@ def context_attention_weights(q, k_cache, v_cache, key_weights, cu_seqlens_q,
         if sinks is not None:
             s = torch.cat([s, sinks.float()[:, None, None].expand(-1, n, 1)],
                           dim=-1)
-        p = torch.softmax(s, dim=-1)[..., :L]
-        p[:, :max(n - L, 0)] = 0        # rows ahead of the first key see none
+        # nothing for keys that a row does not see, whatever its other scores are
+        p = torch.softmax(s, dim=-1)[..., :L].masked_fill(later, 0.)
         out[cs[b]:cs[b + 1]] = (p @ v).transpose(0, 1).to(q.dtype)
         _add_key_weights(key_weights, block_tables[b], L, n, p)
     return out

@@ -706,3 +706,67 @@ def test_rows_behind_the_last_sequence(width):
     ops._K.context_attention_weights(out, q, k, v, w, seq, base, cu, lens, tables,
                                      0.1, torch.empty(0, device="cuda"))
     assert torch.equal(out[:7], own) and (out[7:] == 7).all()
+
+
+@pytest.mark.parametrize("dev", CPU_OR_GPU)
+@pytest.mark.parametrize("layout", [(8, 2, 64), (7, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("width", [None, 240, 3200])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_scores_that_are_no_number(dev, layout, fp8, width, bad):
+    """A row and head with such a score comes out as no number, and so do the entries
+    of the keys that it sees; all others are as ever. The first sequence has it in a
+    query, the last in a key whose share of the keys has scores far below the row's
+    largest."""
+    QH, KH, D = layout
+    G, scale = QH // KH, D ** -0.5
+    new, lens = [6, 3, 2], [66, 10, 952]
+    k, v, w, tables = _pages(lens, KH, D, fp8, width)
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(sum(new), QH, D, generator=g).bfloat16()
+
+    def put(cache, j, x):               # into the last sequence's key j, kv head 0
+        x = torch.tensor(x)
+        cache[tables[2, j // PAGE], 0, j % PAGE, 5] = \
+            x.to(torch.float8_e4m3fn).view(torch.uint8) if fp8 else x.bfloat16()
+
+    q[9:, :, 5] = 64.
+    put(k, 900, 448.)
+    # in 64 bits without what is no number
+    put(k, 3, 0.)
+    want, near, want_w, off = _oracle(q, k, v, w, new, lens, tables, scale, None)
+    put(k, 3, math.nan if fp8 else bad)         # e4m3 has no infinity
+    q[1, 0, 3] = math.nan
+    live = torch.ones(sum(new), QH, dtype=torch.bool)
+    live[1, 0] = False
+    live[9:, :G] = False
+
+    def seen(*n):                       # kv head 0's first keys of a sequence
+        keys = torch.zeros(w.shape, dtype=torch.bool)
+        for b, m in zip((0, 2), n):
+            j = torch.arange(m)
+            keys[tables[b, j // PAGE].long(), 0, j % PAGE] = True
+        return keys
+
+    k, v, q, tables = (t.to(dev) for t in (k, v, q, tables))
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    cu = torch.tensor([0] + new).cumsum(0).int().to(dev)
+    got = w.to(dev)
+    out = ops.context_attention_weights(q, k, v, got, cu, n, tables, scale)
+    out, got = out.cpu().double(), got.cpu().double()
+    assert out[~live].isnan().all()
+    err = (out - want).abs()
+    assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20)[live].all()
+    keys = seen(62, 952)
+    assert got[keys].isnan().all()
+    other = (off > 0) & ~keys
+    assert ((got - want_w).abs() <= off)[other].all()
+    # single tokens: these rows of the three sequences
+    rows = [1, 6, 10]
+    got = w.to(dev)
+    out = ops.paged_attention_weights(q[rows], k, v, got, tables, n, scale)
+    out, got = out.cpu(), got.cpu()
+    assert torch.equal(out.isnan(), ~live[rows, :, None].expand_as(out))
+    keys = seen(66, 952)
+    assert got[keys].isnan().all()
+    assert not got[(off > 0) & ~keys].isnan().any()
