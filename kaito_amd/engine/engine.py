@@ -133,10 +133,10 @@ class LLMEngine:
             raise ValueError(f"kv_budget: no kernels for {group} heads of "
                              f"{m.head_dim} per kv head")
 
-    def _cut_caches(self, seqs: List[Sequence]) -> None:
-        """Cuts the caches that have outgrown cfg.kv_budget, behind the step
-        just launched, and gives their pages back: whoever takes these comes
-        later in the same stream."""
+    def _cut_caches(self, seqs: List[Sequence], decode: bool) -> None:
+        """Cuts the caches that have outgrown cfg.kv_budget, behind the chunks
+        or, with decode, ahead of the token that comes next, and gives their
+        pages back: whoever takes these comes later in the same stream."""
         cfg = self.cfg
         if cfg.kv_budget is None:
             return
@@ -144,7 +144,7 @@ class LLMEngine:
         for seq in seqs:
             if not seq.block_table or seq.status == SeqStatus.FINISHED:
                 continue
-            keys = (seq.sched_len - 1 if seq.sched_len else
+            keys = (seq.sched_tokens - 1 if decode else
                     seq.prefilled_len) - seq.evicted
             if keys > cfg.kv_budget + cfg.kv_budget_slack:
                 cut.append(seq)
@@ -464,14 +464,14 @@ class LLMEngine:
             hidden = self.runner.execute_prefill(batch.chunks)
             samp = self._prefill_bookkeep(batch)
             if not samp:
-                self._cut_caches(batch.seqs)
+                self._cut_caches(batch.seqs, decode=False)
                 return finished          # all chunks partial: no sampling
             tokens, lp = self._sample_prefill_pp(hidden, samp)
             finished += self._commit(samp, tokens.tolist(),
                                      [s.epoch for s in samp],
                                      self._lp_rows([lp + (0,)], len(samp))
                                      if lp is not None else None)
-            self._cut_caches(batch.seqs)
+            self._cut_caches(batch.seqs, decode=False)
             return finished
 
         if self._pp:
@@ -494,6 +494,8 @@ class LLMEngine:
         pend = self._pending
         sampled = pend.tokens if pend is not None else None
         pending_map = (pend.tokens, pend.index) if pend is not None else None
+        # sequences whose keys came from elsewhere have not been cut yet
+        self._cut_caches(batch.seqs, decode=True)
         logits = self.runner.execute(batch, sampled, pending_map)
         tokens, lp_d = self._sample_lp(logits, batch.seqs)
         for seq in batch.seqs:
@@ -514,7 +516,7 @@ class LLMEngine:
             event=event,
             index={s.seq_id: i for i, s in enumerate(batch.seqs)},
             lp_parts=[(lp_d[0], lp_d[1], 0)] if lp_d is not None else [])
-        self._cut_caches(batch.seqs)
+        self._cut_caches(batch.seqs, decode=True)
         # resolve the PREVIOUS step while the GPU runs this one
         finished += self._resolve_pending()
         self._pending = new_pend

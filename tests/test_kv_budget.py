@@ -200,3 +200,49 @@ def test_serving_on_the_gpu(eager, dtype):
     wide = LLMEngine(_cfg(**dict(kw, kv_budget=200))).capture_graphs()
     for s in wide.generate(prompts, short):
         assert s.evicted == 0 and len(s.output_token_ids) == 20
+
+
+def test_transferred_sequences_are_cut_before_they_decode():
+    """100 keys that come from an engine without a budget: none has received
+    anything, so that the newest and the first ones stay."""
+    from kaito_amd.engine.kv_transfer import extract_kv, inject_kv
+    from kaito_amd.engine.sequence import SeqStatus
+    prompt, sp = list(range(10, 110)), SamplingParams(max_tokens=30,
+                                                      ignore_eos=True)
+    pre, dec = LLMEngine(_cfg(kv_budget=None)), LLMEngine(_cfg())
+    src = pre.seqs[pre.add_request(prompt, sp)]
+    pre.step()
+    layers = extract_kv(pre.runner.kv_caches, src.block_table, 100, 16)
+    seq = dec.seqs[dec.add_request(prompt, sp)]
+    dec.scheduler.waiting.remove(seq)
+    seq.block_table = dec.pool.allocate(dec.pool.blocks_needed(102))
+    inject_kv(dec.runner.kv_caches, seq.block_table, layers, 16,
+              dec.runner.key_weights)
+    seq.output_token_ids = list(src.output_token_ids)
+    seq.sched_len, seq.status = 101, SeqStatus.RUNNING
+    dec.scheduler.running.append(seq)
+    while dec.has_unfinished():
+        dec.step()
+    assert seq.evicted > 0 and len(seq.output_token_ids) == 30
+    assert dec.pool.num_free == dec.pool.num_blocks
+
+    lists, model = _Lists(dec.cfg), dec.runner.model
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(LlamaAttention, "attend",
+                  lambda attn, *a: lists.attend(attn, *a))
+        toks, at = list(prompt), 0
+        while len(toks) < 130:
+            T = len(toks) - at
+            meta = AttnMetadata(
+                is_prefill=True, slot_mapping=torch.full((T,), -1),
+                cu_seqlens=torch.tensor([0, T], dtype=torch.int32),
+                max_seqlen=T)
+            hidden = model(torch.tensor(toks[at:]), torch.arange(at, len(toks)),
+                           [None] * model.num_local_layers, meta)
+            at = len(toks)
+            toks.append(int(model.compute_logits(hidden[-1:]).argmax(-1)))
+            if T == 100:
+                for i, (k, v, w) in lists.layers.items():
+                    lists.layers[i] = (k, v, torch.zeros_like(w))
+            lists.cut()
+    assert seq.output_token_ids == toks[100:]
