@@ -92,6 +92,11 @@ class LLMEngine:
                 seq.prompt_token_ids, seq.block_table)
         self.scheduler = Scheduler(cfg, self.pool, restore_cb,
                                    state_pool=self.state_pool)
+        if cfg.kv_budget is not None \
+                and self.scheduler.cut_above < cfg.kv_budget \
+                and cfg.kv_budget < self.runner.max_model_len:
+            raise ValueError(f"kv_budget: {self.pool.num_blocks} pages do not "
+                             f"hold {cfg.kv_budget} keys and the next ones")
         self.sampler = Sampler(cfg.device, cfg.seed)
         from ..parallel.state import get_state
         self._pp = get_state().pp_size > 1
@@ -146,7 +151,7 @@ class LLMEngine:
                 continue
             keys = (seq.sched_tokens - 1 if decode else
                     seq.prefilled_len) - seq.evicted
-            if keys > cfg.kv_budget + cfg.kv_budget_slack:
+            if keys > self.scheduler.cut_above:
                 cut.append(seq)
                 lens.append(keys)
         if not cut:
@@ -155,7 +160,7 @@ class LLMEngine:
                                cfg.kv_budget, cfg.kv_budget_recent)
         for seq, keys in zip(cut, lens):
             seq.evicted += keys - cfg.kv_budget
-            need = self.pool.blocks_needed(seq.sched_tokens + 1 - seq.evicted)
+            need = self.scheduler.pages_of(seq)
             free = seq.block_table[need:]
             seq.block_table = seq.block_table[:need]
             self.pool.free(free)

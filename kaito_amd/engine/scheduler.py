@@ -66,6 +66,12 @@ class Scheduler:
         self.waiting: deque[Sequence] = deque()
         self.prefilling: List[Sequence] = []   # admitted, prompt KV partial
         self.running: List[Sequence] = []
+        # a bounded cache is cut once it holds more keys than this: the budget
+        # and its slack, or all that the pool holds beside the next token's
+        self.cut_above = None
+        if cfg.kv_budget is not None:
+            self.cut_above = min(cfg.kv_budget + cfg.kv_budget_slack,
+                                 pool.num_blocks * pool.block_size - 2)
         # called at admission: restore_cb(seq) -> covered prefix tokens
         self.restore_cb = restore_cb
         # opt-in: admit only prompts that fit the step budget whole
@@ -88,6 +94,24 @@ class Scheduler:
     def add(self, seq: Sequence) -> None:
         seq.status = SeqStatus.WAITING
         self.waiting.append(seq)
+
+    def pages_of(self, seq: Sequence) -> int:
+        """Pages that a sequence has to have: for all of its tokens and the
+        next one, or for as many of them as a bounded cache holds at once, a
+        step's chunk on what is not yet cut."""
+        keys = seq.sched_tokens + 1 - seq.evicted
+        if self.cut_above is not None:
+            keys = min(keys, self.pool.num_blocks * self.pool.block_size,
+                       self.cut_above + self.cfg.max_num_batched_tokens + 1)
+        return self.pool.blocks_needed(keys)
+
+    def _chunk(self, seq: Sequence, budget: int) -> int:
+        """Tokens of a sequence's next chunk."""
+        n = min(seq.num_context_tokens - seq.prefilled_len, budget)
+        if self.cut_above is not None:          # what its pages have room for
+            n = min(n, len(seq.block_table) * self.pool.block_size
+                    - (seq.prefilled_len - seq.evicted))
+        return n
 
     # ---- scheduling ----
     def schedule(self) -> Optional[ScheduledBatch]:
@@ -130,7 +154,7 @@ class Scheduler:
             remaining = seq.num_context_tokens - seq.prefilled_len
             if remaining <= 0:
                 continue
-            n = min(remaining, budget)
+            n = self._chunk(seq, budget)
             chunks.append(PrefillChunk(seq, seq.prefilled_len, n))
             budget -= n
 
@@ -138,7 +162,7 @@ class Scheduler:
         room = self.cfg.max_num_seqs - len(self.running) - len(self.prefilling)
         while self.waiting and room > 0 and budget > 0:
             seq = self.waiting[0]
-            need = self.pool.blocks_needed(seq.num_tokens + 1)
+            need = self.pages_of(seq)
             if not self.pool.can_allocate(need):
                 break
             if self.state_pool is not None:
@@ -173,7 +197,7 @@ class Scheduler:
                 seq.block_table = []
                 seq.status = SeqStatus.WAITING
                 break
-            n = min(remaining, budget)
+            n = self._chunk(seq, budget)
             chunks.append(PrefillChunk(seq, seq.prefilled_len, n))
             self.prefilling.append(seq)
             budget -= n

@@ -246,3 +246,89 @@ def test_transferred_sequences_are_cut_before_they_decode():
                     lists.layers[i] = (k, v, torch.zeros_like(w))
             lists.cut()
     assert seq.output_token_ids == toks[100:]
+
+
+def _drained(eng, steps=3000):
+    for _ in range(steps):
+        if not eng.has_unfinished():
+            return True
+        eng.step()
+        tables = [s.block_table for s in eng.seqs.values()]
+        pages = [p for t in tables for p in t]
+        assert len(set(pages)) == len(pages)
+        assert len(pages) + eng.pool.num_free == eng.pool.num_blocks
+    return False
+
+
+def test_a_preempted_sequence_comes_back(monkeypatch):
+    """102 tokens in three of six pages: preempted there, all of its tokens would
+    need seven. It is computed anew in chunks, cut between them, and what waits
+    behind it has its turn."""
+    eng = LLMEngine(_cfg(num_gpu_blocks=6, kv_budget=16, kv_budget_slack=32,
+                         max_num_seqs=4))
+    prompt = [(7 * i) % 90 + 5 for i in range(71)]
+    long = eng.seqs[eng.add_request(prompt, SP)]
+    while long.num_tokens < 102:
+        eng.step()
+    assert long.evicted > 0
+    others = [eng.add_request([5 + i, 9, 40], SP) for i in range(2)]
+    # the pool runs dry: what a younger sequence's growth does
+    eng.flush()
+    taken = eng.pool.allocate(eng.pool.num_free)
+    for _ in range(40):
+        if long.epoch:
+            break
+        eng.step()
+    assert long.epoch > 0
+    eng.pool.free(taken)
+    assert _drained(eng)
+    for i in (long.seq_id, *others):
+        assert len(eng.seqs[i].output_token_ids) == 60
+    assert eng.pool.num_free == 6
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_small_pools_end(seed):
+    """Random budgets, slacks beyond the pool, chunks and arrivals: every request
+    ends with all of its tokens."""
+    import random
+    rng = random.Random(seed)
+    blocks = rng.randint(3, 9)
+    budget = rng.randint(4, min(60, blocks * 16 - 2))
+    eng = LLMEngine(_cfg(
+        num_gpu_blocks=blocks, kv_budget=budget,
+        kv_budget_recent=rng.randint(0, budget),
+        kv_budget_slack=rng.choice([0, 8, 32, 100]), max_num_seqs=4,
+        max_num_batched_tokens=rng.choice([16, 40, 8192])))
+    want = {}
+    for _ in range(rng.randint(2, 6)):
+        n = rng.choice([1, 5, 30, 90, 150])
+        most = rng.choice([1, 12, 60])
+        sid = eng.add_request([rng.randint(3, 90) for _ in range(n)],
+                              SamplingParams(max_tokens=most, ignore_eos=True))
+        want[sid] = most
+        for _ in range(rng.choice([0, 3, 20])):
+            eng.step()
+    assert _drained(eng)
+    for sid, most in want.items():
+        assert len(eng.seqs[sid].output_token_ids) == most
+
+
+def test_a_prompt_takes_the_pages_of_a_budget_and_a_chunk(monkeypatch):
+    """150 tokens in chunks of 24 through eight pages, the result that of a pool
+    which would hold them all."""
+    prompt = [(11 * i) % 90 + 4 for i in range(150)]
+    small = LLMEngine(_cfg(num_gpu_blocks=8, max_num_batched_tokens=24))
+    sid = small.add_request(prompt, SP)
+    small.step()
+    # 32 + 8 keys, 24 more and the next token
+    assert len(small.seqs[sid].block_table) == -(-65 // 16)
+    assert _drained(small)
+    assert small.seqs[sid].output_token_ids == _replayed(
+        small, prompt, 60, monkeypatch, chunk=24)
+
+
+def test_a_pool_below_the_budget_is_refused():
+    with pytest.raises(ValueError):
+        LLMEngine(_cfg(num_gpu_blocks=2))
+    LLMEngine(_cfg(num_gpu_blocks=2, max_model_len=32))      # nothing is cut
