@@ -569,7 +569,9 @@ class ModelRunner:
     def cut_caches(self, tables: List[List[int]], lens: List[int],
                    budget: int, recent: int) -> None:
         """Cuts the caches of sequences (their pages, their keys) to `budget`
-        keys each, every layer by its own weights, in the current stream."""
+        keys each, every layer by its own weights, in the current stream.
+        What a layer's keys have received is summed over the heads of all
+        tensor-parallel ranks, so that they keep the same ones."""
         from .. import ops
         mb = max(len(t) for t in tables)
         flat = np.zeros((len(tables), mb + 1), dtype=np.int32)
@@ -578,8 +580,17 @@ class ModelRunner:
         flat[:, mb] = lens
         flat = torch.from_numpy(flat).to(self.device)
         table, lens = flat[:, :mb].contiguous(), flat[:, mb].contiguous()
-        for (k, v), w in zip(self.kv_caches, self.key_weights):
-            kept, n = ops.heavy_keys(w, table, lens, budget, recent)
+        totals, rows = self.key_weights, table
+        if ps.get_state().tp_size > 1:
+            pages = table.long()
+            totals = torch.stack([w[pages].double().sum(2)
+                                  for w in self.key_weights])
+            totals = ps.tp_all_reduce(totals).float().flatten(1, 2)
+            totals = totals.unsqueeze(2)        # pages of one head
+            rows = torch.arange(table.numel(), dtype=torch.int32,
+                                device=self.device).view_as(table)
+        for (k, v), w, x in zip(self.kv_caches, self.key_weights, totals):
+            kept, n = ops.heavy_keys(x, rows, lens, budget, recent)
             ops.compact_pages(k, v, w, table, kept, n)
         self._last_ids = []             # the next decode step is built anew
 

@@ -332,3 +332,48 @@ def test_a_pool_below_the_budget_is_refused():
     with pytest.raises(ValueError):
         LLMEngine(_cfg(num_gpu_blocks=2))
     LLMEngine(_cfg(num_gpu_blocks=2, max_model_len=32))      # nothing is cut
+
+
+def _tp_worker(rank, world, port):
+    import os
+    os.environ.update({
+        "MASTER_ADDR": "127.0.0.1", "MASTER_PORT": str(port),
+        "WORLD_SIZE": str(world), "RANK": str(rank), "LOCAL_RANK": str(rank)})
+    from kaito_amd.parallel import one_shot
+    from kaito_amd.parallel import state as ps
+    init_parallel(world, backend="gloo")
+    try:
+        eng = LLMEngine(_cfg(tensor_parallel_size=world))
+        run = eng.runner
+        g = torch.Generator().manual_seed(3)
+        tables, lens = [[5, 9, 2, 7], [1, 0, 3]], [60, 41]
+        ref = []
+        for i, ((k, v), w) in enumerate(zip(run.kv_caches, run.key_weights)):
+            own = w.size(1)
+            # every rank draws all heads and keeps its own
+            full = torch.rand(w.size(0), own * world, 16, generator=g)
+            full[:, 0] *= 3             # heads that matter more than others
+            w.copy_(full[:, rank * own:(rank + 1) * own])
+            for x in (k, v):
+                x.copy_(torch.randn(x.shape, generator=g))
+            t = torch.tensor([r + [0] * (4 - len(r)) for r in tables]).int()
+            kept, n = ops.heavy_keys(full, t, torch.tensor(lens).int(), 32, 8)
+            want = [x.clone() for x in (k, v, w)]
+            ops.compact_pages(*want, t, kept, n)
+            ref.append(want)
+        run.cut_caches(tables, lens, 32, 8)
+        for (k, v), w, want in zip(run.kv_caches, run.key_weights, ref):
+            for x, y in zip((k, v, w), want):
+                assert torch.equal(x, y), "other keys than all heads' weights"
+    finally:
+        one_shot.deactivate()
+        ps.destroy()
+
+
+@pytest.mark.parametrize("world", [2])
+def test_ranks_keep_the_same_keys(world):
+    """Tensor-parallel ranks cut to the keys that all of their heads together
+    gave the most weight."""
+    import torch.multiprocessing as mp
+    mp.start_processes(_tp_worker, args=(world, 29683), nprocs=world, join=True,
+                       start_method="spawn")
