@@ -654,6 +654,7 @@ class LLMEngine:
         self.scheduler.advance_prefill_chunks(batch)
         for c in batch.chunks:
             c.seq.sched_len = c.seq.prefilled_len
+        self._cut_caches(batch.seqs, decode=False)
         if not rows:
             return None
         return self.runner.model.compute_logits(hidden).float()

@@ -298,7 +298,8 @@ class Scheduler:
                     f"portion [{start}, {start + n}) outside the "
                     f"{seq.num_context_tokens} known tokens of seq "
                     f"{seq.seq_id}")
-            need = self.pool.blocks_needed(start + n) - len(seq.block_table)
+            need = self.pool.blocks_needed(start + n - seq.evicted) \
+                - len(seq.block_table)
             if need > 0:
                 seq.block_table.extend(self.pool.allocate(need))
                 seq._bt_dirty = True

@@ -377,3 +377,47 @@ def test_ranks_keep_the_same_keys(world):
     import torch.multiprocessing as mp
     mp.start_processes(_tp_worker, args=(world, 29683), nprocs=world, join=True,
                        start_method="spawn")
+
+
+def test_explicit_steps_are_cut(monkeypatch):
+    """Two requests in portions that the caller composes, cut between them: the
+    logits of plain lists, and no more pages than a budget, its slack and a
+    portion need."""
+    eng = LLMEngine(_cfg())
+    toks = [[(7 * i) % 90 + 4 for i in range(140)],
+            [(5 * i) % 80 + 9 for i in range(70)]]
+    sizes = [[30, 1, 1, 40, 9, 1, 50, 1, 1, 6], [1, 1, 20, 1, 30, 1, 1, 1, 1, 13]]
+    got = [[], []]
+    for a, b in zip(*sizes):
+        for i, n in enumerate((a, b)):
+            at = len(eng.seqs[i].prompt_token_ids) if i in eng.seqs else 0
+            eng.extend_request(i, toks[i][at:at + n])
+        out = eng.step_explicit([(0, a), (1, b)], [(0, a - 1), (1, b - 1)])
+        for i in (0, 1):
+            got[i].append(out[i])
+            seq = eng.seqs[i]
+            assert seq.prefilled_len - seq.evicted <= 40
+            assert len(seq.block_table) <= -(-(41 + 50) // 16)
+    model = eng.runner.model
+    for i in (0, 1):
+        assert eng.seqs[i].evicted > 0
+        lists, at = _Lists(eng.cfg), 0
+        for n, row in zip(sizes[i], got[i]):
+            with monkeypatch.context() as m:
+                m.setattr(LlamaAttention, "attend",
+                          lambda attn, *a: lists.attend(attn, *a))
+                meta = AttnMetadata(
+                    is_prefill=True, slot_mapping=torch.full((n,), -1),
+                    cu_seqlens=torch.tensor([0, n], dtype=torch.int32),
+                    max_seqlen=n)
+                hidden = model(torch.tensor(toks[i][at:at + n]),
+                               torch.arange(at, at + n),
+                               [None] * model.num_local_layers, meta)
+            at += n
+            want = model.compute_logits(hidden[-1:]).float()[0]
+            # bf16 hidden states of other batch sizes round otherwise here and there
+            assert torch.allclose(row, want, atol=0.05, rtol=0.05)
+            lists.cut()
+    for i in (0, 1):
+        eng.release(i)
+    assert eng.pool.num_free == eng.pool.num_blocks
