@@ -551,8 +551,7 @@ class ModelRunner:
             b["block_tables"][:bs].copy_(
                 torch.from_numpy(flat), non_blocking=True)
             if dst:
-                at = torch.tensor([dst, src], dtype=torch.long,
-                                  device=self.device)
+                at = self._upload(np.array([dst, src], dtype=np.int64))
                 b["input_ids"].index_copy_(0, at[0], ptoks[at[1]])
         self._last_ids = ids_now
 
@@ -563,6 +562,13 @@ class ModelRunner:
             g.replay()
             return out[:bs]
         return self._decode_forward(bs)
+
+    def _upload(self, x: np.ndarray) -> torch.Tensor:
+        """x on the device; the host does not wait for what the stream has
+        yet to do."""
+        x = torch.from_numpy(x)
+        return x.pin_memory().to(self.device, non_blocking=True) \
+            if self.is_gpu else x
 
     # ------------------------------------------------------------- budget
     @torch.no_grad()
@@ -578,7 +584,7 @@ class ModelRunner:
         for i, t in enumerate(tables):
             flat[i, :len(t)] = t
         flat[:, mb] = lens
-        flat = torch.from_numpy(flat).to(self.device)
+        flat = self._upload(flat)
         table, lens = flat[:, :mb].contiguous(), flat[:, mb].contiguous()
         totals, rows = self.key_weights, table
         if ps.get_state().tp_size > 1:

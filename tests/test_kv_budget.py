@@ -421,3 +421,29 @@ def test_explicit_steps_are_cut(monkeypatch):
     for i in (0, 1):
         eng.release(i)
     assert eng.pool.num_free == eng.pool.num_blocks
+
+
+@pytest.mark.gpu
+def test_a_cut_does_not_wait_for_the_stream():
+    """A cut and the decode step that is built anew behind it, whose tokens are
+    still under way, are issued while the stream is busy."""
+    eng = LLMEngine(_cfg(device="cuda"))
+    seqs = [eng.seqs[eng.add_request(list(range(a, a + 39)), SP)]
+            for a in (10, 30)]
+    for _ in range(2):
+        eng.step()
+    run, pend = eng.runner, eng._pending
+    assert pend is not None and not seqs[0].evicted
+
+    def launch():
+        run.cut_caches([s.block_table for s in seqs], [40, 40], 32, 8)
+        run.execute_decode(seqs, pend.tokens, (pend.tokens, pend.index))
+
+    launch()                            # what the first launch loads
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(2_000_000_000)
+    done.record()
+    launch()
+    assert not done.query()
+    torch.cuda.synchronize()
