@@ -113,13 +113,18 @@ class ModelRunner:
         else:
             block_bytes = 2 * m.num_layers * kvh * cfg.block_size \
                 * m.head_dim * elem
+        scratch = 0
         if cfg.kv_budget is not None:
             block_bytes += m.num_layers * kvh * cfg.block_size * 4
+            # the scores of a decode step, f32 by the tables' width
+            scratch = cfg.max_num_seqs * (m.num_heads // tp) \
+                * (-(-self._decode_pages() // 2) * 2) * cfg.block_size * 4
         if cfg.num_gpu_blocks is not None:
             n_blocks = cfg.num_gpu_blocks
         elif self.is_gpu:
             free, total = torch.cuda.mem_get_info(self.device)
-            budget = int(total * cfg.gpu_memory_utilization) - (total - free)
+            budget = int(total * cfg.gpu_memory_utilization) \
+                - (total - free) - scratch
             n_blocks = max(budget // block_bytes, 16)
         else:
             n_blocks = 512  # CPU tests
@@ -283,14 +288,18 @@ class ModelRunner:
         return hidden[wide[3 * T:]]
 
     # ------------------------------------------------------------- decode
-    def _init_decode_buffers(self):
-        cfg = self.cfg
-        max_bs = max(max(cfg.graph_batch_sizes), cfg.max_num_seqs)
-        longest = self.max_model_len
+    def _decode_pages(self) -> int:
+        """Width of the decode steps' tables."""
+        cfg, longest = self.cfg, self.max_model_len
         if cfg.kv_budget is not None:   # caches are cut before they decode
             longest = min(longest, cfg.kv_budget + cfg.kv_budget_slack
                           + 2 * cfg.block_size)
-        mb = cfg.max_blocks_per_seq(longest)
+        return cfg.max_blocks_per_seq(longest)
+
+    def _init_decode_buffers(self):
+        cfg = self.cfg
+        max_bs = max(max(cfg.graph_batch_sizes), cfg.max_num_seqs)
+        mb = self._decode_pages()
         dev = self.device
         # the per-row inputs are rows of two blocks, so that a rebuilt batch
         # arrives in one copy each

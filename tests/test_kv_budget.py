@@ -447,3 +447,17 @@ def test_a_cut_does_not_wait_for_the_stream():
     launch()
     assert not done.query()
     torch.cuda.synchronize()
+
+
+def test_the_pool_leaves_room_for_scores(monkeypatch):
+    """Pages take what is left beside the scores of the widest decode step."""
+    eng = LLMEngine(_cfg(max_num_seqs=64, max_model_len=4096, kv_budget=1000))
+    run, m = eng.runner, eng.cfg.model
+    eng.cfg.num_gpu_blocks, run.is_gpu = None, True
+    mem = 30 << 20
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *_: (mem, mem))
+    n = run.profile_and_allocate_kv()
+    page = m.num_layers * m.num_kv_heads * 16 * (2 * 2 * m.head_dim + 4)
+    scores = 64 * m.num_heads * (1008 + 32) * 4
+    room = int(mem * eng.cfg.gpu_memory_utilization) - scores
+    assert 16 < n < 64 * 256 and room - 2 * page < n * page <= room
