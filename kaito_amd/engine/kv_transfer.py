@@ -34,8 +34,13 @@ class KVPayload:
 
 def extract_kv(kv_caches, block_table: List[int], n_tokens: int,
                block_size: int) -> List[Tuple[torch.Tensor, torch.Tensor]]:
-    """Gather a sequence's KV for transfer: [kvh, n_tokens, d] per layer."""
+    """Gather a sequence's KV for transfer: [kvh, n_tokens, d] per layer. Its
+    first n_tokens keys, which a sequence that a kv_budget has cut
+    (Sequence.evicted > 0) does not hold any more."""
     nb = (n_tokens + block_size - 1) // block_size
+    if nb > len(block_table):
+        raise ValueError(f"{n_tokens} tokens are not in {len(block_table)} "
+                         f"pages of {block_size}")
     dev = kv_caches[0][0].device
     blocks = torch.tensor(block_table[:nb], dtype=torch.long, device=dev)
     out = []

@@ -461,3 +461,13 @@ def test_the_pool_leaves_room_for_scores(monkeypatch):
     scores = 64 * m.num_heads * (1008 + 32) * 4
     room = int(mem * eng.cfg.gpu_memory_utilization) - scores
     assert 16 < n < 64 * 256 and room - 2 * page < n * page <= room
+
+
+def test_cut_sequences_are_not_extracted():
+    from kaito_amd.engine.kv_transfer import extract_kv
+    eng = LLMEngine(_cfg(kv_budget_slack=16))
+    seq = eng.seqs[eng.add_request(list(range(5, 54)), SP)]     # 49 keys
+    eng.step()
+    assert seq.evicted > 0
+    with pytest.raises(ValueError):
+        extract_kv(eng.runner.kv_caches, seq.block_table, 49, 16)
