@@ -770,3 +770,99 @@ def test_scores_that_are_no_number(dev, layout, fp8, width, bad):
     keys = seen(66, 952)
     assert got[keys].isnan().all()
     assert not got[(off > 0) & ~keys].isnan().any()
+
+
+# workgroups of 256 keys (128 with 256 dims) from 96 on: whole prompts, whose
+# workgroups begin inside the chunk, at rows that are no multiple of a tile's positions
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [1, 4, 7])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("shared", [True, False])
+def test_whole_prompts(G, D, fp8, shared):
+    """shared: one kv head and a wide table, the first pass in shares of the keys."""
+    if shared:
+        _run("cuda", (G, 1, D), [701, 333], [0, 37], fp8=fp8, sinks=fp8, width=800,
+             seed=G)
+    else:
+        _run("cuda", (8 * G, 8, D), [389, 97, 300, 520, 1], [0, 0, 25, 3, 600],
+             fp8=fp8, sinks=not fp8, seed=G)
+
+
+@pytest.mark.gpu
+def test_many_tiles_of_rows():
+    """Every place of the three buffers of rows, many times over."""
+    _run("cuda", (8, 1, 128), [2100], [130], width=3200, seed=5)
+    _run("cuda", (5, 1, 64), [1500, 700], [0, 0], fp8=True, width=1700, seed=6)
+
+
+# tables of 2049 to 8192 keys, whose totals the choosing launch makes by itself, and of
+# up to 32768, which stay in registers; as many keys to choose among as whole rows of
+# 1024 threads, one less and one more
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,budget,recent", [
+    ([2049, 1500, 2048], 1024, 1),
+    ([4352, 4225, 4096], 4096, 512),
+    ([8192, 8191, 5121], 5000, 1000),
+    ([8193, 8192, 9], 100, 0),
+    ([5120 + 64, 5119 + 64, 5121 + 64], 2000, 64),
+    ([20000, 16384 + 300, 12289 + 300], 9000, 300),
+    ([32768, 32767, 28673], 16384, 1024),
+])
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal"])
+def test_heavy_keys_of_ordinary_caches(lens, budget, recent, kind):
+    pages = -(-max(lens) // PAGE)
+    g = torch.Generator().manual_seed(11)
+    w = torch.rand(pages * len(lens), 8, PAGE, generator=g) ** 4 * 10
+    if kind == "ties":
+        w = (w * 2).floor()
+        w[::3] = 0.5
+    elif kind == "equal":
+        w.fill_(0.25)
+    tables = torch.randperm(len(w), generator=g).int().view(len(lens), pages)
+    kept, n = ops.heavy_keys(w.cuda(), tables.cuda(),
+                             torch.tensor(lens, dtype=torch.int32).cuda(), budget,
+                             recent)
+    assert torch.equal(kept.cpu(), _heavy(w, tables, lens, budget, recent))
+    assert n.tolist() == [min(L, budget) for L in lens]
+
+
+# rows of 64, 128, 256 and 512 bytes, moved whole where there are workgroups enough
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,fp8", [(64, True), (64, False), (128, True),
+                                   (128, False), (256, True), (256, False)])
+def test_compact_pages_of_a_batch(D, fp8):
+    B, KH = 64, 8
+    lens = [300 - 3 * b for b in range(B)]
+    k, v, w, tables = _pages(lens, KH, D, fp8)
+    stay = [min(n, 150 + b) for b, n in enumerate(lens)]
+    kept = torch.full((B, 220), -1, dtype=torch.int32)
+    g = torch.Generator().manual_seed(6)
+    for b, (n, L) in enumerate(zip(stay, lens)):
+        kept[b, :n] = torch.randperm(L, generator=g)[:n].sort().values.int()
+    got = [t.cuda() for t in (k, v, w)]
+    ops.compact_pages(*got, tables.cuda(), kept.cuda(),
+                      torch.tensor(stay, dtype=torch.int32).cuda())
+    _close(k, v, w, tables, kept, stay)
+    for a, b in zip(got, (k, v, w)):
+        assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("layout", [(8, 2, 64), (32, 8, 128), (8, 4, 256)])
+def test_outputs_of_the_plain_operators(layout, fp8):
+    """Keeping weights changes no output where the keys are not shared out
+    otherwise: the same bits as context_attention and paged_attention."""
+    QH, KH, D = layout
+    new, lens = [300, 1, 200, 77] * 24, [310, 40, 200, 700] * 24
+    k, v, w, tables = (t.cuda() for t in _pages(lens, KH, D, fp8))
+    q = torch.randn(sum(new), QH, D).bfloat16().cuda()
+    cu = torch.tensor([0] + new).cumsum(0).int().cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    scale = D ** -0.5
+    got = ops.context_attention_weights(q, k, v, w.clone(), cu, n, tables, scale)
+    assert torch.equal(got, ops.context_attention(q, k, v, cu, n, tables, scale))
+    x = q[:len(lens)]
+    got = ops.paged_attention_weights(x, k, v, w.clone(), tables, n, scale)
+    assert torch.equal(got, ops.paged_attention(x, k, v, tables, n, scale))
