@@ -269,7 +269,9 @@ class EngineConfig:
     # kv_budget_slack keys, every layer is cut to the kv_budget keys that
     # have received the most attention, the newest kv_budget_recent always
     # among them, and the pages behind are given back (None: all are kept).
-    # Keeps prefix caching, host offload and mixed steps off.
+    # Prompts attend to what the pages hold, 8-bit keys too. Keeps prefix
+    # caching and host offload off; mixed steps, pipeline stages, windows and
+    # latent attention are refused.
     kv_budget: Optional[int] = None
     kv_budget_recent: int = 256
     kv_budget_slack: int = 128

@@ -471,3 +471,97 @@ def test_cut_sequences_are_not_extracted():
     assert seq.evicted > 0
     with pytest.raises(ValueError):
         extract_kv(eng.runner.kv_caches, seq.block_table, 49, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eager", [True, False])
+@pytest.mark.parametrize("dtype", ["auto", "fp8"])
+def test_a_budget_that_holds_everything_on_the_gpu(eager, dtype):
+    """The tokens of an engine without a budget, prompts in one chunk and in
+    several. With 8-bit pages in several only: a whole prompt without a budget
+    attends to its keys ahead of their rounding, with one to what the pages hold."""
+    prompts = [list(range(10, 100)), [3, 5, 7, 11], list(range(40, 71))]
+    sp = SamplingParams(max_tokens=40, ignore_eos=True)
+    for chunk in (8192, 32) if dtype == "auto" else (32,):
+        kw = dict(device="cuda", enforce_eager=eager, kv_cache_dtype=dtype,
+                  graph_batch_sizes=(1, 2, 4), max_num_seqs=4,
+                  max_num_batched_tokens=chunk)
+        want = LLMEngine(_cfg(**dict(kw, kv_budget=None))).capture_graphs()
+        got = LLMEngine(_cfg(**dict(kw, kv_budget=200))).capture_graphs()
+        for a, b in zip(want.generate(prompts, sp), got.generate(prompts, sp)):
+            assert a.output_token_ids == b.output_token_ids and b.evicted == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["auto", "fp8"])
+def test_every_call_of_a_served_batch(dtype, monkeypatch):
+    """Every attention, choice and closing that the engine asks for, cuts at
+    unlike steps among them, against 64 bits over what the pages held; and every
+    sequence's tables and lengths against its positions and its cuts."""
+    import test_key_weights as kw
+    eng = LLMEngine(_cfg(device="cuda", kv_cache_dtype=dtype, max_num_seqs=4,
+                         max_num_batched_tokens=48))
+    calls = dict.fromkeys(("chunk", "token", "choose", "close"), 0)
+    real = {n: getattr(ops, n) for n in (
+        "context_attention_weights", "paged_attention_weights", "heavy_keys",
+        "compact_pages")}
+
+    def check(out, q, k, v, w, before, new, lens, tables, scale, sinks):
+        want, near, want_w, off = kw._oracle(
+            q, k, v, before, new, lens, tables,
+            scale, None if sinks is None else sinks.cpu())
+        err = (out.cpu().double() - want).abs()
+        assert (err <= 2.0 ** -8 * (want.abs() + near) + 2.0 ** -20).all()
+        live = off > 0
+        now = w.cpu()
+        assert ((now.double() - want_w).abs() <= off)[live].all()
+        assert torch.equal(now[~live], before[~live])
+
+    def chunk(q, k, v, w, cu, lens, tables, scale, sinks=None, tiles=None):
+        calls["chunk"] += 1
+        before = w.cpu()
+        out = real["context_attention_weights"](q, k, v, w, cu, lens, tables,
+                                                scale, sinks, tiles)
+        check(out, q, k, v, w, before, (cu[1:] - cu[:-1]).tolist(), lens.tolist(),
+              tables, scale, sinks)
+        return out
+
+    def token(q, k, v, w, tables, lens, scale, sinks=None):
+        calls["token"] += 1
+        before = w.cpu()
+        out = real["paged_attention_weights"](q, k, v, w, tables, lens, scale, sinks)
+        seqs = eng.scheduler.running[:len(q)]
+        assert lens.tolist() == [s.sched_tokens - s.evicted for s in seqs]
+        for s, row in zip(seqs, tables.tolist()):
+            assert row[:len(s.block_table)] == s.block_table
+        check(out, q, k, v, w, before, [1] * len(q), lens.tolist(), tables, scale,
+              sinks)
+        return out
+
+    def choose(w, tables, lens, budget, recent):
+        calls["choose"] += 1
+        kept, n = real["heavy_keys"](w, tables, lens, budget, recent)
+        assert torch.equal(kept.cpu(), kw._heavy(w.cpu(), tables.cpu(),
+                                                 lens.tolist(), budget, recent))
+        return kept, n
+
+    def close(k, v, w, tables, kept, n):
+        calls["close"] += 1
+        ref = [t.cpu() for t in (k, v, w)]
+        real["compact_pages"](k, v, w, tables, kept, n)
+        kw._close(*ref, tables.cpu(), kept.cpu(), n.tolist())
+        for a, b in zip((k, v, w), ref):
+            assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+
+    for name, f in zip(real, (chunk, token, choose, close)):
+        monkeypatch.setattr(ops, name, f)
+    ids = [eng.add_request(list(range(a, a + n)), SP)
+           for a, n in ((10, 90), (30, 20), (50, 35))]
+    while eng.has_unfinished():
+        eng.step()
+    layers = eng.cfg.model.num_layers
+    assert all(eng.seqs[i].evicted > 0 for i in ids)
+    # the three are cut at different steps, and the long prompt between its chunks
+    assert calls["choose"] == calls["close"] >= 8 * layers
+    assert calls["chunk"] >= 3 * layers and calls["token"] >= 59 * layers
+    assert eng.pool.num_free == eng.pool.num_blocks
