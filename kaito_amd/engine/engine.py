@@ -93,8 +93,8 @@ class LLMEngine:
         self.scheduler = Scheduler(cfg, self.pool, restore_cb,
                                    state_pool=self.state_pool)
         if cfg.kv_budget is not None \
-                and self.scheduler.cut_above < cfg.kv_budget \
-                and cfg.kv_budget < self.runner.max_model_len:
+                and self.pool.num_blocks * cfg.block_size - 2 \
+                < cfg.kv_budget < self.runner.max_model_len:
             raise ValueError(f"kv_budget: {self.pool.num_blocks} pages do not "
                              f"hold {cfg.kv_budget} keys and the next ones")
         self.sampler = Sampler(cfg.device, cfg.seed)

@@ -70,8 +70,9 @@ class Scheduler:
         # and its slack, or all that the pool holds beside the next token's
         self.cut_above = None
         if cfg.kv_budget is not None:
-            self.cut_above = min(cfg.kv_budget + cfg.kv_budget_slack,
-                                 pool.num_blocks * pool.block_size - 2)
+            self.cut_above = max(cfg.kv_budget, min(
+                cfg.kv_budget + cfg.kv_budget_slack,
+                pool.num_blocks * pool.block_size - 2))
         # called at admission: restore_cb(seq) -> covered prefix tokens
         self.restore_cb = restore_cb
         # opt-in: admit only prompts that fit the step budget whole

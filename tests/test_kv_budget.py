@@ -334,6 +334,16 @@ def test_a_pool_below_the_budget_is_refused():
     LLMEngine(_cfg(num_gpu_blocks=2, max_model_len=32))      # nothing is cut
 
 
+@pytest.mark.parametrize("n", [29, 30, 31])
+def test_a_sequence_that_fills_a_pool_of_no_budget_is_not_cut(n):
+    eng = LLMEngine(_cfg(num_gpu_blocks=2, max_model_len=32, kv_budget=40))
+    out = eng.generate([list(range(5, 5 + n))], SP)[0]
+    want = LLMEngine(_cfg(kv_budget=None, max_model_len=32)).generate(
+        [list(range(5, 5 + n))], SP)[0]
+    assert out.evicted == 0 and out.output_token_ids == want.output_token_ids
+    assert eng.pool.num_free == 2
+
+
 def _tp_worker(rank, world, port):
     import os
     os.environ.update({
