@@ -984,7 +984,8 @@ def context_attention_weights(q: torch.Tensor, k_cache: torch.Tensor,
     that ends before them) comes out as zeros. A score that is no number, or
     infinite, makes its row's output NaN and the entries of all keys that the
     row sees. Pages are a sequence's own here: what becomes of the weights of one
-    that two tables of a call share is not defined. q bf16 of any strides, head
+    that two tables of a call share is not defined. q bf16 of any strides (a row
+    2^25 elements behind the last at most), head
     sizes 64, 128 and 256, bf16 or e4m3 pages of 16 keys."""
     if q.is_cuda:
         q = _query_rows(q)

@@ -15,16 +15,24 @@
 // are per-lane scalars and a weight is a multiply-add, an exponential and a
 // multiply-add into its key's sum.
 //
-// What bounds it: the matrix unit's power. With operands of random bits the chip
-// takes 33.6 ns for a product of 32 x 32 x 16 on a SIMD, twice the 16.3 ns that
-// constant operands take (1.0 PFLOP/s); 2048 rows of 32 heads over 16384 keys and 8
-// kv heads of 128 are 261 us of such products, and the pass takes 268, beside 566 of
+// What bounds it: its products of 32 x 32 x 16. With operands of random bits one takes
+// 33.6 ns on a SIMD (16.3 with constant ones): 2048 rows of 32 heads over 16384 keys
+// and 8 kv heads of 128 are 261 us of them, and the pass takes 268, beside 566 of
 // flash_prefill.h's twice as many. One product after another and then all weights
 // 381 us; the loop without masks and addresses 315; products and weights in turns
 // 298; tiles of 64 rows and fragments four products ahead of their use 268. Eight
-// waves that share a tile: 278. Products of 16 x 16 x 32, of which two take 18 ns by
-// themselves and as many multiply-adds and exponentials in between 25: 287 (276 with
-// those gathered by fours), without copies and barriers 258, without LDS reads 222.
+// waves that share a tile: 278. It is not what the matrix unit can do: two products
+// of 16 x 16 x 32, the same operations, take 18 ns with random operands and 25 with
+// as many multiply-adds and exponentials in between. In this loop they took 287 (276
+// with those gathered by fours), without copies and barriers 258, without LDS reads
+// 222: there, staging and the reads of fragments are ahead of them.
+//
+// Weights enter the product with V as bf16, as in context_attention, and the outputs
+// are its bits wherever the keys are not shared out. As value and remainder, the EXT
+// form, the long chunk took 974 us for both passes instead of 785, eight of 97 to 1000
+// rows 505 (423), four of 333 to 1200 over e4m3 pages and heads of 64 773 (630); the
+// error against 64 bits was 1.7e-3 instead of 1.9e-3, of which the rounding of the
+// output is 1.65e-3. Scores, maxima, sums and the keys' weights are f32.
 #include "flash_prefill.h"
 #include "keys_common.h"
 #include <torch/library.h>
@@ -572,10 +580,15 @@ void context_attention_weights(at::Tensor out, at::Tensor q, at::Tensor k_cache,
     auto blocks = [&](const int keys) {
       return dim3((held + keys - 1) / keys * a.KH, B);
     };
-    // Both in us, 256 keys a workgroup (64 shared): 512 rows of 4 heads on 512 keys,
-    // 16 workgroups, 41.5 and 22.5; on 1024 64 and 31; 1024 on 2048 98 and 54; four
-    // of 512 on 1024, 128 workgroups, 42.4 and 45.3; 1024 on 5120, 160, 75 and 115;
-    // 16 on 16016 12.1 and 42.8.
+    // Both passes in us, by 256 keys a workgroup (128 with 256 dims) and by shared 64
+    // (32), at 64 and 128 workgroups of the former. 32/8 heads of 128, 128 rows 46.0
+    // and 40.7, 58.5 and 64.8, 1024 rows 136 and 105, 170 and 174; 28/4 of 128, 1024
+    // rows 248 and 188, 362 and 358; 32/32 of 64, 128 rows 32.5 and 28.7, 33.1 and
+    // 34.8; 8/4 of 256, 1024 rows 120 and 117, 151 and 182. At 192 shared ones lose by
+    // up to 37 %, but for groups of 8 heads of 64, which would rather share up to
+    // there: 1024 rows 161 and 93, 202 and 169, at 192 243 and 242. The table's width
+    // stands for the lengths, which are on the device: where sequences are much
+    // shorter, workgroups of the first kind are left without keys.
     if (blocks(KEYS).x * B < 96)
       hipLaunchKernelGGL((key_weight_few_kernel<D_, F_>), blocks(SHARED),
                          dim3(512), 0, stream, w);
